@@ -1,0 +1,153 @@
+// What the attention kernels share: element types, warp-level matrix products on 16-bit operands, asynchronous 16-byte copies into
+// shared memory, and the argument checks that their launchers have in common.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace mf {
+namespace attn {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ uint32_t SmemAddr32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// 16 bytes global -> shared, asynchronously; with `bytes` 0 nothing is read and the place is filled with zeros.
+__device__ __forceinline__ void CpAsync16(uint32_t dst, const void *src, uint32_t bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void CpCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void CpWait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void LdMatrix4(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void LdMatrix4T(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+// c[16 x 8] += a[16 x 16] b[16 x 8], fp32 sums.
+template <typename T>
+__device__ __forceinline__ void Mma16x8x16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void Mma16x8x16<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void Mma16x8x16<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Two floats rounded to a pair of T, `lo` in the low half.
+template <typename T>
+__device__ __forceinline__ uint32_t Pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t Pack2<__nv_bfloat16>(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <>
+__device__ __forceinline__ uint32_t Pack2<__half>(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ float2 Unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 Unpack2<__nv_bfloat16>(uint32_t v)
+{
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 Unpack2<__half>(uint32_t v)
+{
+    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+}
+
+// Two e4m3 values (low 16 bits) as a pair of fp16, which holds all of them exactly.
+__device__ __forceinline__ uint32_t E4m3ToHalf2(uint32_t v)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)v));
+    return r;
+}
+
+// 2^x to about two units in the last place of fp32; -inf gives 0.
+__device__ __forceinline__ float Exp2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// One row of attention by one warp, key by key: for rows whose result is not finite. In a tile product a masked key counts 0 * v, which is
+// not 0 where v is infinite or NaN; here only the keys below `seen` are touched. q: the row's query, out: its place.
+template <typename T, int D>
+__device__ __noinline__ void AttendRow(const T *q, const T *k, long long kStep, const T *v, long long vStep, int seen, float factor, T *out, float *lse)
+{
+    constexpr int kMine = D / 64;  // pairs of columns of a lane
+    const int lane = threadIdx.x & 31;
+    float x[2 * kMine], acc[2 * kMine], top = -INFINITY, sum = 0;
+#pragma unroll
+    for (int i = 0; i < kMine; i++) {
+        const float2 p = Unpack2<T>(*(const uint32_t *)(q + i * 64 + lane * 2));
+        x[2 * i] = p.x, x[2 * i + 1] = p.y;
+        acc[2 * i] = acc[2 * i + 1] = 0;
+    }
+    for (int j = 0; j < seen; j++) {
+        float s = 0;
+#pragma unroll
+        for (int i = 0; i < kMine; i++) {
+            const float2 p = Unpack2<T>(*(const uint32_t *)(k + j * kStep + i * 64 + lane * 2));
+            s += x[2 * i] * p.x + x[2 * i + 1] * p.y;
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+            s += __shfl_xor_sync(~0u, s, d);
+        }
+        s *= factor;
+        const float best = fmaxf(top, s), base = best == -INFINITY ? 0.0f : best, shrink = Exp2(top - base), p = Exp2(s - base);
+        top = best;
+        sum = sum * shrink + p;
+#pragma unroll
+        for (int i = 0; i < kMine; i++) {
+            const float2 y = Unpack2<T>(*(const uint32_t *)(v + j * vStep + i * 64 + lane * 2));
+            acc[2 * i] = acc[2 * i] * shrink + p * y.x;
+            acc[2 * i + 1] = acc[2 * i + 1] * shrink + p * y.y;
+        }
+    }
+    const float scale = sum != 0 ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMine; i++) {
+        *(uint32_t *)(out + i * 64 + lane * 2) = Pack2<T>(acc[2 * i] * scale, acc[2 * i + 1] * scale);
+    }
+    if (lse != nullptr && lane == 0) {
+        *lse = top * kLn2 + logf(sum);
+    }
+}
+
+}  // namespace attn
+}  // namespace mf

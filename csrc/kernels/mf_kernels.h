@@ -241,6 +241,108 @@ int mf_k_reshard(const mf_reshard_args_t *argsDev, int nEmulatedRanks, int rankC
 // may be NULL) caps the number of rows actually processed.
 int mf_k_quant_rows_fp8(const void *x, void *q, float *scale, int rows, int K, const int *rowLimit, mf_stream_t stream);
 
+// ------------------------------------------------------------------------------------------------ attention
+
+enum { MF_K_BF16 = 0, MF_K_FP16 = 1, MF_K_E4M3 = 2 };
+
+// One new token per sequence over a paged cache. q, out: [B][kvHeads * group][D] with the given strides (elements; D contiguous). k, v:
+// [pages][kvHeads][pageSize][D] with the same strides, `stride` = {page, head, slot}. table: [tableRows][tableWidth] page numbers, row
+// stride tableStride; lengths: [tableRows]; rows: [B] or NULL: the table row (and length) of each sequence. Lengths are clamped to
+// [0, tableWidth * pageSize]; a sequence without keys gives zeros and an lse of -inf. Page numbers outside [0, pages) that a length
+// reaches, and rows outside the table, read nothing (the keys count as zeros, the sequence as empty) and set *status to MF_DEV_ERR_BOUNDS.
+// kScale, vScale: [kvHeads] fp32, for e4m3 caches. lse: [B][kvHeads * group] fp32 or NULL, natural logarithm. All addresses and
+// strides are multiples of 16 bytes. D: 64 or 128; the cache has the query's type, or e4m3.
+typedef struct {
+    const void *q;
+    const void *k;
+    const void *v;
+    const int *table;
+    const int *lengths;
+    const int *rows;
+    const float *kScale;
+    const float *vScale;
+    void *out;
+    float *lse;
+    int *status;
+    void *workspace;  // mf_k_decode_attention_workspace() bytes of this call's own
+    void *marks;      // set by the launcher
+    long long qStride[2];
+    long long outStride[2];
+    long long stride[3];
+    long long tableStride;
+    int B, kvHeads, group, pageSize, pages, tableWidth, tableRows;
+    float scale;
+} mf_decode_attention_args_t;
+size_t mf_k_decode_attention_workspace(int B, int kvHeads, int group, int D, long long capacity);
+int mf_k_decode_attention(const mf_decode_attention_args_t *args, int D, int qType, int cacheType, mf_stream_t stream);
+
+// Prompts packed one behind the other. q, out: [tokensQ][kvHeads * group][D], k, v: [tokensK][kvHeads][D], strides {token, head} in elements,
+// D contiguous. Sequence b has query rows [cuQ[b], cuQ[b + 1]) and keys [cuK[b], cuK[b + 1]); with `causal` its row i sees the keys up to
+// i + (keys - rows). Rows that see no key give zeros and an lse of -inf; rows outside [cuQ[0], cuQ[B]) are left alone. cuQ and cuK must
+// ascend; what they say beyond the tokens is cut off. All addresses and strides are multiples of 16 bytes. D: 64 or 128.
+typedef struct {
+    const void *q;
+    const void *k;
+    const void *v;
+    const int *cuQ;
+    const int *cuK;
+    void *out;
+    float *lse;  // [tokensQ][kvHeads * group] or NULL
+    long long qStride[2];
+    long long kStride[2];
+    long long vStride[2];
+    long long outStride[2];
+    int B, kvHeads, group, tokensQ, tokensK, causal;
+    float scale;
+} mf_prefill_attention_args_t;
+int mf_k_prefill_attention(const mf_prefill_attention_args_t *args, int D, int type, mf_stream_t stream);
+
+// ------------------------------------------------------------------------------------------------ paged key-value cache
+
+enum { MF_KV_MAX_SEQS = 1 << 18 };
+
+// A cache: data [layers][pages][2 (key, value)][kvHeads][pageSize][rowBytes], table [seqs][tableWidth] page numbers (-1: none), lengths [seqs],
+// refs [pages]: how many sequences hold a page, 0 = free. status: device int that receives MF_DEV_ERR_BOUNDS. data and refs are 16-byte
+// aligned, rowBytes is a multiple of 16; everything is contiguous.
+typedef struct {
+    void *data;
+    int *table;
+    int *lengths;
+    int *refs;
+    int *status;
+    int layers, pages, pageSize, kvHeads, rowBytes, seqs, tableWidth;
+} mf_kv_cache_t;
+
+// Keys and values of `tokens` tokens, [tokens][kvHeads][dim] with strides {token, head} in elements, into the slots (page * pageSize + place in
+// the page) of one layer's pages, which `data` points to. Slots below 0 are left out, slots behind the last page too, with the status
+// set. One slot named twice gets one of the two rows. e4m3: x * (1 / scale of the head), rounded to nearest, saturated.
+typedef struct {
+    const void *k;
+    const void *v;
+    const long long *slots;
+    const float *kScale;
+    const float *vScale;
+    void *data;
+    int *status;
+    long long kStride[2];
+    long long vStride[2];
+    int tokens, kvHeads, dim, pages, pageSize;
+} mf_kv_write_args_t;
+int mf_k_kv_write(const mf_kv_write_args_t *args, int srcType, int cacheType, mf_stream_t stream);
+
+// Lengthens the sequences rows[i] by counts[i] tokens and writes the slots of the new tokens, request by request; slots behind the last one
+// become -1. All or nothing: with too few free pages, more than `room` tokens, a table row that is too short, a row out of range or
+// named twice, all slots are -1, the cache is as before and the status is set. n <= seqs.
+size_t mf_k_kv_reserve_workspace(int n, long long room, int pageSize);
+int mf_k_kv_reserve(const mf_kv_cache_t *cache, const int *rows, const int *counts, int n, long long room, long long *slots, void *workspace, mf_stream_t stream);
+// dst[i], an empty sequence, gets the length and the pages of src[i]. A pair that is out of range, whose destination is in use, named before or a
+// source of this call is left out and sets the status. n <= seqs.
+int mf_k_kv_fork(const mf_kv_cache_t *cache, const int *src, const int *dst, int n, mf_stream_t stream);
+int mf_k_kv_free(const mf_kv_cache_t *cache, const int *rows, int n, mf_stream_t stream);
+// remap [pages]: the new number of each page that is in use, -1 for the others.
+size_t mf_k_kv_compact_workspace(int pages);
+int mf_k_kv_compact(const mf_kv_cache_t *cache, int *remap, void *workspace, mf_stream_t stream);
+
 // ------------------------------------------------------------------------------------------------ test support (K7)
 
 // dst[i] = hash(seed, i) for i in [0, n) bytes; deterministic on host and device (see mf_k_pattern_byte_host).

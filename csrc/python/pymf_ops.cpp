@@ -291,6 +291,114 @@ void BindOps(py::module_ &m)
             }
             return rc == MF_K_OK ? p.Combine(epochC, stream) : rc;
         });
+    ops.attr("BF16") = (int)MF_K_BF16;
+    ops.attr("FP16") = (int)MF_K_FP16;
+    ops.attr("E4M3") = (int)MF_K_E4M3;
+    ops.attr("KV_MAX_SEQS") = (int)MF_KV_MAX_SEQS;
+    ops.def("decode_attention_workspace", &mf_k_decode_attention_workspace, py::arg("B"), py::arg("kv_heads"), py::arg("group"), py::arg("D"),
+            py::arg("capacity"));
+    ops.def("decode_attention", [](uint64_t q, uint64_t k, uint64_t v, uint64_t table, uint64_t lengths, uint64_t rows, uint64_t kScale, uint64_t vScale,
+                                   uint64_t out, uint64_t lse, uint64_t status, uint64_t workspace, int64_t qs0, int64_t qs1, int64_t os0, int64_t os1,
+                                   int64_t s0, int64_t s1, int64_t s2, int64_t tableStride, int B, int kvHeads, int group, int pageSize, int pages,
+                                   int tableWidth, int tableRows, float scale, int D, int qType, int cacheType, uint64_t stream) {
+        mf_decode_attention_args_t a{};
+        a.q = (const void *)q;
+        a.k = (const void *)k;
+        a.v = (const void *)v;
+        a.table = (const int *)table;
+        a.lengths = (const int *)lengths;
+        a.rows = (const int *)rows;
+        a.kScale = (const float *)kScale;
+        a.vScale = (const float *)vScale;
+        a.out = (void *)out;
+        a.lse = (float *)lse;
+        a.status = (int *)status;
+        a.workspace = (void *)workspace;
+        a.qStride[0] = qs0;
+        a.qStride[1] = qs1;
+        a.outStride[0] = os0;
+        a.outStride[1] = os1;
+        a.stride[0] = s0;
+        a.stride[1] = s1;
+        a.stride[2] = s2;
+        a.tableStride = tableStride;
+        a.B = B;
+        a.kvHeads = kvHeads;
+        a.group = group;
+        a.pageSize = pageSize;
+        a.pages = pages;
+        a.tableWidth = tableWidth;
+        a.tableRows = tableRows;
+        a.scale = scale;
+        return mf_k_decode_attention(&a, D, qType, cacheType, (mf_stream_t)stream);
+    });
+    ops.def("prefill_attention", [](uint64_t q, uint64_t k, uint64_t v, uint64_t cuQ, uint64_t cuK, uint64_t out, uint64_t lse, int64_t qs0, int64_t qs1,
+                                    int64_t ks0, int64_t ks1, int64_t vs0, int64_t vs1, int64_t os0, int64_t os1, int B, int kvHeads, int group, int tokensQ,
+                                    int tokensK, int causal, float scale, int D, int type, uint64_t stream) {
+        mf_prefill_attention_args_t a{};
+        a.q = (const void *)q;
+        a.k = (const void *)k;
+        a.v = (const void *)v;
+        a.cuQ = (const int *)cuQ;
+        a.cuK = (const int *)cuK;
+        a.out = (void *)out;
+        a.lse = (float *)lse;
+        a.qStride[0] = qs0;
+        a.qStride[1] = qs1;
+        a.kStride[0] = ks0;
+        a.kStride[1] = ks1;
+        a.vStride[0] = vs0;
+        a.vStride[1] = vs1;
+        a.outStride[0] = os0;
+        a.outStride[1] = os1;
+        a.B = B;
+        a.kvHeads = kvHeads;
+        a.group = group;
+        a.tokensQ = tokensQ;
+        a.tokensK = tokensK;
+        a.causal = causal;
+        a.scale = scale;
+        return mf_k_prefill_attention(&a, D, type, (mf_stream_t)stream);
+    });
+    // The tensors of a paged key-value cache, and the launches on it.
+    py::class_<mf_kv_cache_t>(ops, "KvCache")
+        .def(py::init([](uint64_t data, uint64_t table, uint64_t lengths, uint64_t refs, uint64_t status, int layers, int pages, int pageSize, int kvHeads,
+                         int rowBytes, int seqs, int tableWidth) {
+            return mf_kv_cache_t{(void *)data, (int *)table, (int *)lengths, (int *)refs, (int *)status, layers, pages, pageSize, kvHeads, rowBytes, seqs, tableWidth};
+        }))
+        .def("write", [](const mf_kv_cache_t &c, int layer, uint64_t k, uint64_t v, uint64_t slots, uint64_t kScale, uint64_t vScale, int64_t ks0, int64_t ks1,
+                         int64_t vs0, int64_t vs1, int tokens, int dim, int srcType, int cacheType, uint64_t stream) {
+            mf_kv_write_args_t a{};
+            a.k = (const void *)k;
+            a.v = (const void *)v;
+            a.slots = (const long long *)slots;
+            a.kScale = (const float *)kScale;
+            a.vScale = (const float *)vScale;
+            a.data = (unsigned char *)c.data + (size_t)layer * c.pages * 2 * c.kvHeads * c.pageSize * c.rowBytes;
+            a.status = c.status;
+            a.kStride[0] = ks0;
+            a.kStride[1] = ks1;
+            a.vStride[0] = vs0;
+            a.vStride[1] = vs1;
+            a.tokens = tokens;
+            a.kvHeads = c.kvHeads;
+            a.dim = dim;
+            a.pages = c.pages;
+            a.pageSize = c.pageSize;
+            return mf_k_kv_write(&a, srcType, cacheType, (mf_stream_t)stream);
+        })
+        .def("reserve_workspace", [](const mf_kv_cache_t &c, int n, int64_t room) { return mf_k_kv_reserve_workspace(n, room, c.pageSize); })
+        .def("reserve", [](const mf_kv_cache_t &c, uint64_t rows, uint64_t counts, int n, int64_t room, uint64_t slots, uint64_t ws, uint64_t stream) {
+            return mf_k_kv_reserve(&c, (const int *)rows, (const int *)counts, n, room, (long long *)slots, (void *)ws, (mf_stream_t)stream);
+        })
+        .def("fork", [](const mf_kv_cache_t &c, uint64_t src, uint64_t dst, int n, uint64_t stream) {
+            return mf_k_kv_fork(&c, (const int *)src, (const int *)dst, n, (mf_stream_t)stream);
+        })
+        .def("free", [](const mf_kv_cache_t &c, uint64_t rows, int n, uint64_t stream) { return mf_k_kv_free(&c, (const int *)rows, n, (mf_stream_t)stream); })
+        .def("compact_workspace", [](const mf_kv_cache_t &c) { return mf_k_kv_compact_workspace(c.pages); })
+        .def("compact", [](const mf_kv_cache_t &c, uint64_t remap, uint64_t ws, uint64_t stream) {
+            return mf_k_kv_compact(&c, (int *)remap, (void *)ws, (mf_stream_t)stream);
+        });
     ops.def("allreduce_rmsnorm", [](uint64_t argsDev, int nEmulated, int rankCount, int T, int H, float eps, int algo, uint32_t channel, uint64_t epoch,
                                     uint64_t timeoutNs, int ctas, uint64_t stream) {
         return mf_k_allreduce_rmsnorm((const mf_allreduce_args_t *)argsDev, nEmulated, rankCount, T, H, eps, algo, channel, epoch, timeoutNs, ctas,
