@@ -13,6 +13,15 @@ namespace attn {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+template <typename T>
+struct Bf16 {
+    static constexpr bool value = false;
+};
+template <>
+struct Bf16<__nv_bfloat16> {
+    static constexpr bool value = true;
+};
+
 __device__ __forceinline__ uint32_t SmemAddr32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 // 16 bytes global -> shared, asynchronously; with `bytes` 0 nothing is read and the place is filled with zeros.

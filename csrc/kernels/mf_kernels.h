@@ -287,7 +287,8 @@ typedef struct {
     const int *cuQ;
     const int *cuK;
     void *out;
-    float *lse;  // [tokensQ][kvHeads * group] or NULL
+    float *lse;   // [tokensQ][kvHeads * group] or NULL
+    int *status;  // or NULL: MF_K_GEMM_PIPELINE_EXPIRED where a bounded wait ran out
     long long qStride[2];
     long long kStride[2];
     long long vStride[2];

@@ -135,6 +135,13 @@ __device__ __forceinline__ void TmaLoad2D(void *smemDst, const CUtensorMap *m, u
                  "l"((uint64_t)m), "r"(SmemAddr(bar)), "r"(c0), "r"(c1)
                  : "memory");
 }
+// The same for a 3-D tensor map (c0 innermost).
+__device__ __forceinline__ void TmaLoad3D(void *smemDst, const CUtensorMap *m, uint64_t *bar, int c0, int c1, int c2)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(SmemAddr(smemDst)),
+                 "l"((uint64_t)m), "r"(SmemAddr(bar)), "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
+}
 // The same for a 4-D tensor map (c0 innermost).
 __device__ __forceinline__ void TmaLoad4D(void *smemDst, const CUtensorMap *m, uint64_t *bar, int c0, int c1, int c2, int c3)
 {
@@ -195,6 +202,29 @@ __device__ __forceinline__ void TmemLdWait16(float *v)
                  : "memory");
 }
 
+// The same with the 32 values of TmemLd32Issue.
+__device__ __forceinline__ void TmemLdWait32(float *v)
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
+                   "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
+                   "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+                 :
+                 : "memory");
+}
+// Stores to 16 consecutive columns of this thread's TMEM lane; complete after TmemStWait().
+__device__ __forceinline__ void TmemSt16(uint32_t taddr, const uint32_t *v)
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]),
+        "r"(v[14]), "r"(v[15]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void TmemStWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
 // 32 consecutive fp32 columns of this thread's TMEM lane, waited for.
 __device__ __forceinline__ void TmemLd32(uint32_t taddr, float *v)
 {
@@ -238,6 +268,38 @@ __host__ __device__ constexpr uint32_t InstrDescF8(uint32_t m, uint32_t n) { ret
 __host__ __device__ constexpr uint32_t InstrDescBf16(uint32_t m, uint32_t n)
 {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+// The same for a tile whose rows run along K, the matrix's other dimension (64 16-bit values, 128 bytes, swizzled) being contiguous: groups of eight
+// rows are 1024 bytes apart, the next 64 values of the contiguous dimension `next64` bytes.
+__device__ __forceinline__ uint64_t SmemDescSw128Transposed(uint32_t smemByteAddr, uint32_t next64)
+{
+    return SmemDescSw128(smemByteAddr) | (uint64_t)(next64 >> 4) << 16;
+}
+// kind::f16 with fp16 (format 0) or bf16 (1) operands of one type; `transposedB`: B as SmemDescSw128Transposed describes it.
+__host__ __device__ constexpr uint32_t InstrDescF16(uint32_t m, uint32_t n, bool bf16, bool transposedB)
+{
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((transposedB ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+// D[tmem] (+)= A[smem] * B[smem] over 16 values of K, issued by ONE thread. accumulate = 0 overwrites D.
+__device__ __forceinline__ void MmaF16(uint32_t tmemD, uint64_t aDesc, uint64_t bDesc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmemD),
+        "l"(aDesc), "l"(bDesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// The same with A in TMEM: two values of K to a 32-bit column, row r in lane r.
+__device__ __forceinline__ void MmaF16Tmem(uint32_t tmemD, uint32_t tmemA, uint64_t bDesc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n.reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmemD),
+        "r"(tmemA), "l"(bDesc), "r"(idesc), "r"(accumulate)
+        : "memory");
 }
 
 // D[tmem] (+)= A[smem] * B[smem], issued by ONE thread. accumulate = 0 overwrites D.

@@ -332,7 +332,7 @@ void BindOps(py::module_ &m)
         a.scale = scale;
         return mf_k_decode_attention(&a, D, qType, cacheType, (mf_stream_t)stream);
     });
-    ops.def("prefill_attention", [](uint64_t q, uint64_t k, uint64_t v, uint64_t cuQ, uint64_t cuK, uint64_t out, uint64_t lse, int64_t qs0, int64_t qs1,
+    ops.def("prefill_attention", [](uint64_t q, uint64_t k, uint64_t v, uint64_t cuQ, uint64_t cuK, uint64_t out, uint64_t lse, uint64_t status, int64_t qs0, int64_t qs1,
                                     int64_t ks0, int64_t ks1, int64_t vs0, int64_t vs1, int64_t os0, int64_t os1, int B, int kvHeads, int group, int tokensQ,
                                     int tokensK, int causal, float scale, int D, int type, uint64_t stream) {
         mf_prefill_attention_args_t a{};
@@ -343,6 +343,7 @@ void BindOps(py::module_ &m)
         a.cuK = (const int *)cuK;
         a.out = (void *)out;
         a.lse = (float *)lse;
+        a.status = (int *)status;
         a.qStride[0] = qs0;
         a.qStride[1] = qs1;
         a.kStride[0] = ks0;

@@ -177,14 +177,15 @@ def decode_attention(q, k_pages, v_pages, table, lengths, *, rows=None, scale=No
     return (out, lse) if isinstance(lse, torch.Tensor) else out
 
 
-def prefill_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, out=None, lse=None, stream=None):
+def prefill_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, out=None, lse=None, status=None, stream=None):
     """Attention of packed prompts. q [tokens, heads, dim], k and v [keys, kv_heads, dim] (any strides, rows contiguous), heads a multiple of
     kv_heads; cu_q int32 [B + 1]: the rows of sequence b are cu_q[b] to cu_q[b + 1], ascending from 0 or more; cu_k the same for keys,
     by default cu_q. With `causal` the last row of a sequence sees all of its keys, each row before it one less: a chunk of a prompt is given as
     its rows with all keys up to its end. scale: of the logits, 1 / sqrt(dim) by default.
 
     Returns out [tokens, heads, dim]; with lse=True (or a tensor for it) also the logarithm of the sum of exponentials, fp32
-    [tokens, heads]. Rows that see no key give zeros and -inf; rows that belong to no sequence are left as they are."""
+    [tokens, heads]. Rows that see no key give zeros and -inf; rows that belong to no sequence are left as they are. status: int32 tensor of one
+    element, receives GEMM_PIPELINE_EXPIRED (3) if a bounded wait inside the kernel ran out."""
     import torch
 
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[2] != q.shape[2]:
@@ -203,16 +204,21 @@ def prefill_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, out=
     _int32("cu_k", cu_k, 1)
     if cu_q.shape[0] < 1 or cu_k.shape != cu_q.shape:
         raise ValueError("cu_q and cu_k have one entry more than there are sequences")
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1):
+        raise ValueError("status must be an int32 tensor of one element")
     _check_out(out, lse, (tokens, heads))
     factor = _scale(scale, dim)
     qs, ks, vs = strides("q", q, 0, 1), strides("k", k, 0, 1), strides("v", v, 0, 1)
+    for t, step in ((q, qs), (k, ks), (v, vs)):
+        if any(n > 1 and s == 0 for n, s in zip(t.shape, step)):
+            raise ValueError("q, k and v must not be expanded: the rows are fetched by strides of their own")
     no_gradient(q, k, v)
-    on_gpu(q, k=k, v=v, cu_q=cu_q, cu_k=cu_k, out=out, lse=lse if isinstance(lse, torch.Tensor) else None)
+    on_gpu(q, k=k, v=v, cu_q=cu_q, cu_k=cu_k, out=out, lse=lse if isinstance(lse, torch.Tensor) else None, status=status)
     with launch_on(q.device, stream):
         given, (out, lse) = out, _result(out, q, lse, (tokens, heads))
         os = strides("out", out, 0, 1) if given is not None else (heads * dim, dim)
         rc = _ops.prefill_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(),
-                                    lse.data_ptr() if isinstance(lse, torch.Tensor) else 0, *qs, *ks, *vs, *os, cu_q.shape[0] - 1, kv_heads, heads // kv_heads,
+                                    lse.data_ptr() if isinstance(lse, torch.Tensor) else 0, status.data_ptr() if status is not None else 0, *qs, *ks, *vs, *os, cu_q.shape[0] - 1, kv_heads, heads // kv_heads,
                                     tokens, keys, int(causal), factor, dim, kind, current_stream_handle())
     if rc != 0:
         raise RuntimeError(f"prefill_attention launch failed ({rc})")
