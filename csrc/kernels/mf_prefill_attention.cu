@@ -3,9 +3,8 @@
 //     out[i, h] = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(s q[i, h] . k_j - m_i),   j <= i + (keys - rows) of i's sequence,
 //
 // in one pass over the keys with a running reference m and sum per row. A CTA takes two tiles of 128 rows, which share the keys and
-// values that stream through shared memory, one pair of 128 keys at a time. The rows of a tile are (token, head of a group): as many
-// query heads of one key head as there are in the largest power of two that divides the group, so that short prompts fill tiles and a
-// causal tile spans few tokens.
+// values that stream through shared memory, one pair of 128 keys at a time. The rows of a tile are (token, head of a group), all
+// query heads of one key head where that fills a tile well, so that short prompts fill tiles and a causal tile spans few tokens.
 //
 //   warps 0-3, 4-7   softmax of the first, of the second tile: a row per thread. S from TMEM, p back over it (16 bits), the sum in a
 //                    register; at the end O from TMEM, divided and stored.
@@ -34,9 +33,19 @@ using namespace mf::attn;
 using namespace mf::sm100;
 
 constexpr int kTile = 128;  // rows of a tile, keys of a tile
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;
 constexpr uint32_t kHalf = kTile * 128;  // bytes of 64 columns of a tile
 constexpr float kSlack = 8.0f;           // powers of two by which the reference may lag behind the maximum
+constexpr int kEarly = 96;               // keys whose P is handed over while the others are still computed
+// Registers of a softmax thread, which holds a row of S, and of the others: 256 * 200 + 128 * 96 of the 384 * 168 of the launch.
+constexpr int kSoftmaxRegs = 200, kOtherRegs = 96;
+
+// What the scheduler warp says about a CTA's next two row tiles.
+struct Work {
+    int q0, rows, t0;   // first query row of the sequence, their number, first token of the tiles
+    int k0, keys, n;    // first key, their number, key tiles to go through; n < 0: no more work
+    int kvh, h0;
+};
 
 template <int D>
 struct Shared {
@@ -44,7 +53,8 @@ struct Shared {
     static constexpr uint32_t kTileBytes = (D / 64) * kHalf;
     unsigned char q[2][kTileBytes];
     unsigned char kv[kStages][kTileBytes];
-    uint64_t qFull, kvFull[kStages], kvEmpty[kStages], sFull[2], pFull[2], oFull[2];
+    uint64_t qFull, qEmpty, kvFull[kStages], kvEmpty[kStages], sFull[2], pFull[2], pRest[2], oFull[2], workFull[2], workEmpty[2];
+    Work work[2];
     uint32_t tmem;
     int abortFlag;
 };
@@ -52,9 +62,11 @@ struct Shared {
 struct Params {
     mf_prefill_attention_args_t a;
     int pack;      // heads in a tile's rows
-    int tokens;    // tokens of a CTA: 256 / pack
+    int tokens;    // tokens of two tiles: 2 * (128 / pack)
+    int wide;      // output rows begin at multiples of 32 bytes: whole sectors are stored
     int headTiles; // kvHeads * group / pack
     int tiles;     // numbers of row tiles, empty ones among them
+    int units;     // tiles * headTiles
 };
 
 __device__ __forceinline__ float Max3(float a, float b, float c)
@@ -63,6 +75,99 @@ __device__ __forceinline__ float Max3(float a, float b, float c)
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+__device__ __forceinline__ uint64_t Both(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 Apart(uint64_t v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t Fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t Add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float AtLeast(float x, float least)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(least));
+    return r;
+}
+
+// 2^x for x <= 16 on the FMA pipe, for a share of the weights: the special function unit gives 16 results a cycle and SM, as long a time for a
+// tile as its MMAs take at D = 128. x = n + f with n the nearest whole number (W. J. Cody, W. Waite, "Software Manual for the Elementary
+// Functions", 1980), 2^f by the polynomial of least relative error on [-1/2, 1/2] (Remez exchange; 7.5e-5 of degree 3, 2.7e-6 of degree 4,
+// below the rounding of p to bf16 and fp16), n added to its exponent. Below -126 the result stays near 2^-126 (the exponent field must not fall below 0); NaN comes out as an
+// infinite or huge p, which has the row computed again.
+template <bool BF16>
+__device__ __forceinline__ float2 Exp2Poly(uint64_t x2)
+{
+    const float2 x = Apart(x2);
+    x2 = Both(AtLeast(x.x, -126.0f), AtLeast(x.y, -126.0f));
+    const uint64_t r2 = Add2(x2, Both(12582912.0f, 12582912.0f));  // 1.5 * 2^23: n stands in the lowest bits
+    const uint64_t f2 = Fma2(Add2(r2, Both(-12582912.0f, -12582912.0f)), Both(-1.0f, -1.0f), x2);
+    uint64_t p2;
+    if (BF16) {
+        p2 = Fma2(Both(0.055171669f, 0.055171669f), f2, Both(0.242611122f, 0.242611122f));
+        p2 = Fma2(p2, f2, Both(0.693260985f, 0.693260985f));
+        p2 = Fma2(p2, f2, Both(0.999928074f, 0.999928074f));
+    } else {
+        p2 = Fma2(Both(0.009570102f, 0.009570102f), f2, Both(0.055917860f, 0.055917860f));
+        p2 = Fma2(p2, f2, Both(0.240247448f, 0.240247448f));
+        p2 = Fma2(p2, f2, Both(0.693121815f, 0.693121815f));
+        p2 = Fma2(p2, f2, Both(0.999999261f, 0.999999261f));
+    }
+    const float2 r = Apart(r2), p = Apart(p2);
+    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(r.x) << 23)), __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23)));
+}
+
+// Of four pairs of weights, how many go to the FMA pipe.
+template <int D>
+struct Poly {
+    static constexpr int kOf4 = 1;
+};
+
+template <int REGS>
+__device__ __forceinline__ void MoreRegisters()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int REGS>
+__device__ __forceinline__ void FewerRegisters()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+
+// A warp's view of the work list: the next two row tiles, or false at its end.
+template <int D>
+struct Worker {
+    int k{0};
+    __device__ __forceinline__ bool Next(Shared<D> &s, volatile int *abortFlag, Work &w)
+    {
+        if (!MbarWaitWarp(&s.workFull[k & 1], (k >> 1) & 1, abortFlag)) {
+            return false;
+        }
+        w = s.work[k & 1];
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) {
+            MbarArrive(&s.workEmpty[k & 1]);
+        }
+        k++;
+        return w.n >= 0;
+    }
+};
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -74,41 +179,28 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
     extern __shared__ unsigned char smemRaw[];
     X &s = *reinterpret_cast<X *>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~(uintptr_t)1023);
     const mf_prefill_attention_args_t &a = p.a;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    GridDependency();
-
-    // Row tiles of sequence b have numbers from cuQ[b] / tokens + b on: enough for its rows wherever they begin, some numbers stay empty. The
-    // last tiles of a causal prompt are the longest, so numbers are handed out from the end.
-    const int tile = p.tiles - 1 - blockIdx.x / p.headTiles, ht = blockIdx.x % p.headTiles;
-    int lo = 0, hi = a.B;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        (a.cuQ[mid] / p.tokens + mid <= tile ? lo : hi) = mid;
-    }
-    const int q0 = a.cuQ[lo], rows = min(a.cuQ[lo + 1], a.tokensQ) - q0, t0 = (tile - (q0 / p.tokens + lo)) * p.tokens;
-    if (q0 < 0 || t0 < 0 || t0 >= rows) {
-        return;
-    }
-    const int k0 = a.cuK[lo], keys = k0 < 0 ? 0 : min(a.cuK[lo + 1], a.tokensK) - k0, past = keys - rows;
-    const int perKv = a.group / p.pack, kvh = ht / perKv, h0 = kvh * a.group + (ht % perKv) * p.pack;
-    const int last = min(rows, t0 + p.tokens);  // token behind the CTA's last one
-    const int see = a.causal ? min(keys, last + past) : keys, n = see > 0 ? (see + kTile - 1) / kTile : 0;
-    const int half = p.tokens / 2;
-    const bool two = t0 + half < rows;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = p.tokens / 2;
 
     if (threadIdx.x == 0) {
         MbarInit(&s.qFull, 1);
+        MbarInit(&s.qEmpty, 2);
         for (int i = 0; i < X::kStages; i++) {
             MbarInit(&s.kvFull[i], 1);
-            MbarInit(&s.kvEmpty[i], 1);
+            MbarInit(&s.kvEmpty[i], 2);
         }
         for (int i = 0; i < 2; i++) {
             MbarInit(&s.sFull[i], 1);
             MbarInit(&s.pFull[i], 4);
+            MbarInit(&s.pRest[i], 4);
             MbarInit(&s.oFull[i], 1);
+            MbarInit(&s.workFull[i], 1);
+            MbarInit(&s.workEmpty[i], 11);
         }
         s.abortFlag = 0;
         MbarInitFence();
+        TmaPrefetchDesc(&mapQ);
+        TmaPrefetchDesc(&mapK);
+        TmaPrefetchDesc(&mapV);
     }
     if (warp == 8) {
         TmemAlloc(&s.tmem, 512);
@@ -118,130 +210,249 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
     TcFenceAfter();
     const uint32_t tmem = s.tmem;
     volatile int *abortFlag = &s.abortFlag;
-    // TMEM columns: S (and P) of the two tiles, then O
-    constexpr uint32_t kO = 2 * kTile;
+    constexpr uint32_t kO = 2 * kTile;  // TMEM columns: S (and P) of the two tiles, then O
+    GridDependency();  // what stands above ran under the end of the kernel before
 
-    if (warp == 9) {
-        const bool elected = ElectOne();
-        if (n > 0 && elected) {
-            MbarExpectTx(&s.qFull, (two ? 2 : 1) * X::kTileBytes);
-            for (int i = 0; i < (two ? 2 : 1); i++) {
-                for (int c = 0; c < D / 64; c++) {
-                    TmaLoad3D(s.q[i] + c * kHalf, &mapQ, &s.qFull, c * 64, h0, q0 + t0 + i * half);
+    if (warp >= 8) {
+        FewerRegisters<kOtherRegs>();
+        if (warp == 10) {
+            // ------------------------------------------------------------------ scheduler
+            // Row tiles of sequence b have numbers from cuQ[b] / tokens + b on: enough for its rows wherever they begin, some numbers stay empty. The
+            // last tiles of a causal prompt are the longest, so numbers are dealt out from the end, there and back over the CTAs.
+            int k = 0;
+            for (int round = 0;; round++) {
+                const long long unit = (long long)round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                const bool end = (long long)round * gridDim.x >= p.units;
+                Work w = {0, 0, 0, 0, 0, -1, 0, 0};
+                if (!end) {
+                    if (unit >= p.units) {
+                        continue;
+                    }
+                    const int tile = p.tiles - 1 - (int)(unit / p.headTiles), ht = (int)(unit % p.headTiles);
+                    int lo = 0, hi = a.B;  // the last sequence whose first number is not behind `tile`: 32 places at a time
+                    while (hi - lo > 1) {
+                        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+                        const unsigned low = __ballot_sync(~0u, at < hi && a.cuQ[at] / p.tokens + at <= tile) | 1u;
+                        const int last = 31 - __clz(low);
+                        hi = min(hi, lo + (last + 1) * step);
+                        lo += last * step;
+                    }
+                    w.q0 = a.cuQ[lo];
+                    w.rows = min(a.cuQ[lo + 1], a.tokensQ) - w.q0;
+                    w.t0 = (tile - (w.q0 / p.tokens + lo)) * p.tokens;
+                    if (w.q0 < 0 || w.t0 < 0 || w.t0 >= w.rows) {
+                        continue;
+                    }
+                    w.k0 = a.cuK[lo];
+                    w.keys = w.k0 < 0 ? 0 : min(a.cuK[lo + 1], a.tokensK) - w.k0;
+                    const int see = a.causal ? min(w.keys, min(w.rows, w.t0 + p.tokens) + w.keys - w.rows) : w.keys;
+                    w.n = see > 0 ? (see + kTile - 1) / kTile : 0;
+                    const int perKv = a.group / p.pack;
+                    w.kvh = ht / perKv;
+                    w.h0 = w.kvh * a.group + (ht % perKv) * p.pack;
+                }
+                if (!MbarWaitWarp(&s.workEmpty[k & 1], ((k >> 1) & 1) ^ 1, abortFlag)) {
+                    break;
+                }
+                if (lane == 0) {
+                    s.work[k & 1] = w;
+                    MbarArrive(&s.workFull[k & 1]);
+                }
+                k++;
+                if (end) {
+                    break;
                 }
             }
-        }
-        uint32_t st = 0, ph = 0;
-        int issued = 0;
-        for (int i = 0; i < 2 * n; i++) {
-            if (!MbarWaitWarp(&s.kvEmpty[st], ph ^ 1, abortFlag)) {
-                break;
-            }
-            if (elected) {
-                MbarExpectTx(&s.kvFull[st], X::kTileBytes);
-                for (int c = 0; c < D / 64; c++) {
-                    TmaLoad3D(s.kv[st] + c * kHalf, i & 1 ? &mapV : &mapK, &s.kvFull[st], c * 64, kvh, k0 + (i >> 1) * kTile);
+        } else if (warp == 9) {
+            // ------------------------------------------------------------------ TMA producer
+            const bool elected = ElectOne();
+            Worker<D> worker;
+            Work w;
+            uint32_t st = 0, ph = 0, qPh = 0;
+            long long issued = 0;
+            bool ok = true, qOpen = false;
+            while (ok && worker.Next(s, abortFlag, w)) {
+                if (w.n == 0) {
+                    continue;
+                }
+                const bool two = w.t0 + half < w.rows;
+                ok = MbarWaitWarp(&s.qEmpty, qPh ^ 1, abortFlag);
+                if (!ok) {
+                    break;
+                }
+                if (elected) {
+                    MbarExpectTx(&s.qFull, (two ? 2 : 1) * (D / 64) * 128 * p.pack * half);
+                    for (int i = 0; i < (two ? 2 : 1); i++) {
+                        for (int c = 0; c < D / 64; c++) {
+                            TmaLoad3D(s.q[i] + c * kHalf, &mapQ, &s.qFull, c * 64, w.h0, w.q0 + w.t0 + i * half);
+                        }
+                    }
+                }
+                qOpen = true;
+                qPh ^= 1;
+                for (int i = 0; i < 2 * w.n; i++) {
+                    ok = MbarWaitWarp(&s.kvEmpty[st], ph ^ 1, abortFlag);
+                    if (!ok) {
+                        break;
+                    }
+                    if (elected) {
+                        MbarExpectTx(&s.kvFull[st], X::kTileBytes);
+                        for (int c = 0; c < D / 64; c++) {
+                            TmaLoad3D(s.kv[st] + c * kHalf, i & 1 ? &mapV : &mapK, &s.kvFull[st], c * 64, w.kvh, w.k0 + (i >> 1) * kTile);
+                        }
+                    }
+                    issued++;
+                    if (++st == X::kStages) {
+                        st = 0;
+                        ph ^= 1;
+                    }
                 }
             }
-            issued++;
-            if (++st == X::kStages) {
-                st = 0;
-                ph ^= 1;
+            if (*abortFlag != 0) {  // nothing may land in the shared memory of a CTA that has left
+                int own = 0;
+                if (qOpen) {
+                    MbarWaitBounded(&s.qFull, qPh ^ 1, &own);
+                }
+                for (long long i = issued > X::kStages ? issued - X::kStages : 0; i < issued; i++) {
+                    MbarWaitBounded(&s.kvFull[i % X::kStages], (uint32_t)(i / X::kStages) & 1, &own);
+                }
             }
-        }
-        if (*abortFlag != 0 && n > 0) {  // nothing may land in the shared memory of a CTA that has left
-            int own = 0;
-            MbarWaitBounded(&s.qFull, 0, &own);
-            for (int i = max(0, issued - X::kStages); i < issued; i++) {
-                MbarWaitBounded(&s.kvFull[i % X::kStages], (i / X::kStages) & 1, &own);
-            }
-        }
-    } else if (warp == 8) {
-        const bool elected = ElectOne();
-        const uint32_t base = __reduce_or_sync(~0u, tmem);
-        const uint64_t qDesc = SmemDescSw128(SmemAddr(s.q[0])), kDesc = SmemDescSw128(SmemAddr(s.kv[0])), vDesc = SmemDescSw128Transposed(SmemAddr(s.kv[0]), kHalf);
-        constexpr uint32_t iS = InstrDescF16(kTile, kTile, kBf16, false), iO = InstrDescF16(kTile, D, kBf16, true);
-        auto scores = [&](int i, uint32_t stage) {  // S of tile i
+        } else {
+            // ------------------------------------------------------------------ MMA issuers, one for each tile
+            // Everything that the loops and operands go by comes out of a warp reduction: the compiler then knows that it is the same in all lanes and
+            // keeps descriptors in uniform registers.
+            const bool elected = ElectOne();
+            const int i = __reduce_max_sync(~0u, warp == 8 ? 0 : 1);
+            const uint32_t base = __reduce_or_sync(~0u, tmem), sAt = base + i * kTile, oAt = base + kO + i * D;
+            const uint64_t qDesc = SmemDescSw128(SmemAddr(s.q[0])) + i * (X::kTileBytes >> 4), kDesc = SmemDescSw128(SmemAddr(s.kv[0])),
+                           vDesc = SmemDescSw128Transposed(SmemAddr(s.kv[0]), kHalf);
+            constexpr uint32_t iS = InstrDescF16(kTile, kTile, kBf16, false), iO = InstrDescF16(kTile, D, kBf16, true);
+            auto scores = [&](uint32_t stage) {
+                const uint64_t k0 = kDesc + stage * (X::kTileBytes >> 4);
 #pragma unroll
-            for (int k = 0; k < D / 16; k++) {
-                const uint32_t off = (k / 4) * (kHalf >> 4) + (k % 4) * 2;
-                MmaF16(base + i * kTile, qDesc + i * (X::kTileBytes >> 4) + off, kDesc + stage * (X::kTileBytes >> 4) + off, iS, k > 0);
-            }
-        };
-        auto values = [&](int i, uint32_t stage, bool more) {  // O of tile i
-#pragma unroll
-            for (int k = 0; k < kTile / 16; k++) {
-                MmaF16Tmem(base + kO + i * D, base + i * kTile + k * 8, vDesc + stage * (X::kTileBytes >> 4) + k * 128, iO, more || k > 0);
-            }
-        };
-        uint32_t st = 0, ph = 0;
-        auto step = [&]() {
-            if (++st == X::kStages) {
-                st = 0;
-                ph ^= 1;
-            }
-        };
-        bool ok = n > 0 && MbarWaitWarp(&s.qFull, 0, abortFlag) && MbarWaitWarp(&s.kvFull[0], 0, abortFlag);
-        if (ok) {
-            TcFenceAfter();
-            if (elected) {
-                scores(0, 0);
-                MmaCommit(&s.sFull[0]);
-                if (two) {
-                    scores(1, 0);
-                    MmaCommit(&s.sFull[1]);
+                for (int k = 0; k < D / 16; k++) {
+                    const uint32_t off = (k / 4) * (kHalf >> 4) + (k % 4) * 2;
+                    MmaF16(sAt, qDesc + off, k0 + off, iS, k > 0);
                 }
-                MmaCommit(&s.kvEmpty[0]);
-            }
-            step();
-        }
-        for (int j = 0; ok && j < n; j++) {
-            const uint32_t v = st, vPh = ph;
-            step();
-            const uint32_t k = st, kPh = ph;
-            const bool next = j + 1 < n;
-            if (next) {
-                step();
-            }
-            ok = MbarWaitWarp(&s.kvFull[v], vPh, abortFlag) && (!next || MbarWaitWarp(&s.kvFull[k], kPh, abortFlag));
-            for (int i = 0; ok && i < (two ? 2 : 1); i++) {
-                ok = MbarWaitWarp(&s.pFull[i], j & 1, abortFlag);
+            };
+            auto values = [&](uint32_t stage, bool more, int k0, int k1) {  // of the keys [k0, k1)
+                const uint64_t v0 = vDesc + stage * (X::kTileBytes >> 4);
+#pragma unroll
+                for (int k = k0 / 16; k < k1 / 16; k++) {
+                    MmaF16Tmem(oAt, sAt + k * 8, v0 + k * 128, iO, more || k > 0);
+                }
+            };
+            Worker<D> worker;
+            Work w;
+            uint32_t st = 0, ph = 0, qPh = 0, pPh = 0;
+            auto step = [&]() {
+                if (++st == X::kStages) {
+                    st = 0;
+                    ph ^= 1;
+                }
+            };
+            bool ok = true;
+            while (ok && __any_sync(~0u, worker.Next(s, abortFlag, w))) {
+                const int n = __reduce_max_sync(~0u, w.n);
+                if (n == 0) {
+                    continue;
+                }
+                ok = MbarWaitWarp(&s.qFull, qPh, abortFlag);
+                qPh ^= 1;
+                if (__any_sync(~0u, i == 1 && w.t0 + half >= w.rows)) {  // no second tile: its share of the stages is given back at once
+                    if (ok && elected) {
+                        MbarArrive(&s.qEmpty);
+                    }
+                    for (int j = 0; ok && j < 2 * n; j++) {
+                        ok = MbarWaitWarp(&s.kvFull[st], ph, abortFlag);
+                        if (ok && elected) {
+                            MbarArrive(&s.kvEmpty[st]);
+                        }
+                        step();
+                    }
+                    continue;
+                }
+                ok = ok && MbarWaitWarp(&s.kvFull[st], ph, abortFlag);
                 if (!ok) {
                     break;
                 }
                 TcFenceAfter();
                 if (elected) {
-                    values(i, v, j > 0);
-                    if (i == 1 || !two) {
-                        MmaCommit(&s.kvEmpty[v]);
+                    scores(st);
+                    MmaCommit(&s.sFull[i]);
+                    MmaCommit(&s.kvEmpty[st]);
+                    if (n == 1) {
+                        MmaCommit(&s.qEmpty);
                     }
+                }
+                step();
+                for (int j = 0; j < n; j++) {
+                    const uint32_t v = st, vPh = ph;
+                    step();
+                    const uint32_t k = st, kPh = ph;
+                    const bool next = j + 1 < n;
                     if (next) {
-                        scores(i, k);
-                        MmaCommit(&s.sFull[i]);
-                        if (i == 1 || !two) {
+                        step();
+                    }
+                    ok = MbarWaitWarp(&s.kvFull[v], vPh, abortFlag) && (!next || MbarWaitWarp(&s.kvFull[k], kPh, abortFlag)) &&
+                         MbarWaitWarp(&s.pFull[i], pPh, abortFlag);
+                    if (!ok) {
+                        break;
+                    }
+                    TcFenceAfter();
+                    if (elected) {
+                        values(v, j > 0, 0, kEarly);
+                    }
+                    ok = MbarWaitWarp(&s.pRest[i], pPh, abortFlag);
+                    if (!ok) {
+                        break;
+                    }
+                    pPh ^= 1;
+                    TcFenceAfter();
+                    if (elected) {
+                        values(v, true, kEarly, kTile);
+                        if (next) {
+                            scores(k);
+                            MmaCommit(&s.sFull[i]);
                             MmaCommit(&s.kvEmpty[k]);
+                            if (j + 2 == n) {
+                                MmaCommit(&s.qEmpty);
+                            }
+                        } else {
+                            MmaCommit(&s.oFull[i]);
                         }
-                    } else {
-                        MmaCommit(&s.oFull[i]);
+                        MmaCommit(&s.kvEmpty[v]);
                     }
                 }
             }
         }
     } else {
+        // ---------------------------------------------------------------------- softmax
+        MoreRegisters<kSoftmaxRegs>();
         const int i = warp >> 2;  // the tile
-        const int row = (warp & 3) * 32 + lane, token = t0 + i * half + row / p.pack, head = h0 + row % p.pack;
+        const int row = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, sAt = tmem + lanes + i * kTile, oAt = tmem + lanes + kO + i * D;
-        if (i == 0 || two) {
-            const int limit = a.causal ? min(keys, token + past + 1) : keys;  // keys that the row sees
+        const float factor = a.scale * kLog2e;
+        Worker<D> worker;
+        Work w;
+        uint32_t sPh = 0, oPh = 0;
+        bool ok = true;
+        while (ok && worker.Next(s, abortFlag, w)) {
+            if (i == 1 && w.t0 + half >= w.rows) {
+                continue;
+            }
+            // rows that the packing leaves over hold anything, and nobody looks at them
+            const int token = row < p.pack * half ? w.t0 + i * half + row / p.pack : 0x7fffffff, past = w.keys - w.rows;
+            const bool valid = token < w.rows;
+            const int limit = a.causal && valid ? min(w.keys, token + past + 1) : w.keys;  // keys that the row sees
             const int sure = __reduce_min_sync(~0u, limit);
-            const float factor = a.scale * kLog2e;
             float top = -INFINITY, sum = 0;
-            bool ok = true;
-            for (int j = 0; j < n; j++) {
-                if (!__all_sync(~0u, MbarWaitBounded(&s.sFull[i], j & 1, abortFlag))) {
+            for (int j = 0; j < w.n; j++) {
+                if (!MbarWaitWarp(&s.sFull[i], sPh, abortFlag)) {
                     ok = false;
                     break;
                 }
+                sPh ^= 1;
                 TcFenceAfter();
                 float x[kTile];
 #pragma unroll
@@ -271,7 +482,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                 for (int e = 0; e < 4; e++) {
                     m[e] = fmaxf(m[e], x[kTile - 4 + e]);
                 }
-                const float best = Max3(Max3(m[0], m[1], m[2]), m[3], m[3]);
+                const float best = Max3(fmaxf(m[0], m[1]), m[2], m[3]);
                 const bool grown = (best - top) * factor > kSlack;
                 if (__any_sync(~0u, grown)) {
                     const float shrink = grown ? Exp2((top - best) * factor) : 1.0f;
@@ -292,74 +503,98 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                     }
                 }
                 const float from = top == -INFINITY ? 0.0f : -top * factor;
-                float part[4] = {0, 0, 0, 0};
+                const uint64_t factor2 = Both(factor, factor), from2 = Both(from, from);
+                uint64_t part[2] = {0, 0};
 #pragma unroll
                 for (int c = 0; c < kTile; c += 32) {
-                    uint32_t w[16];
+                    uint32_t w16[16];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const float u = Exp2(fmaf(x[c + e], factor, from)), v = Exp2(fmaf(x[c + e + 1], factor, from));
-                        part[e & 2] += u;
-                        part[(e & 2) + 1] += v;
-                        w[e / 2] = Pack2<T>(u, v);
+                    for (int e = 0; e < 16; e++) {
+                        const uint64_t y = Fma2(Both(x[c + 2 * e], x[c + 2 * e + 1]), factor2, from2);
+                        float2 u;
+                        if (e % 4 < Poly<D>::kOf4) {
+                            u = Exp2Poly<kBf16>(y);
+                        } else {
+                            u = Apart(y);
+                            u = make_float2(Exp2(u.x), Exp2(u.y));
+                        }
+                        part[e & 1] = Add2(part[e & 1], Both(u.x, u.y));
+                        w16[e] = Pack2<T>(u.x, u.y);
                     }
-                    TmemSt16(sAt + c / 2, w);
+                    TmemSt16(sAt + c / 2, w16);
+                    if (c + 32 == kEarly || c + 32 == kTile) {
+                        TmemStWait();
+                        TcFenceBefore();
+                        __syncwarp();
+                        if (lane == 0) {
+                            MbarArrive(c + 32 == kEarly ? &s.pFull[i] : &s.pRest[i]);
+                        }
+                    }
                 }
-                sum += (part[0] + part[1]) + (part[2] + part[3]);
-                TmemStWait();
-                TcFenceBefore();
-                __syncwarp();
-                if (lane == 0) {
-                    MbarArrive(&s.pFull[i]);
-                }
+                const float2 both = Apart(Add2(part[0], part[1]));
+                sum += both.x + both.y;
             }
-            if (n > 0 && ok) {
-                ok = __all_sync(~0u, MbarWaitBounded(&s.oFull[i], 0, abortFlag));
+            if (!ok) {
+                break;
+            }
+            if (w.n > 0) {
+                if (!MbarWaitWarp(&s.oFull[i], oPh, abortFlag)) {
+                    break;
+                }
+                oPh ^= 1;
                 TcFenceAfter();
             }
-            if (ok) {
-                const float scale = sum != 0 ? 1.0f / sum : 0.0f;
-                const size_t at = (size_t)(q0 + token);
-                T *out = (T *)a.out + at * a.outStride[0] + (size_t)head * a.outStride[1];
-                float *lse = a.lse != nullptr ? a.lse + at * a.kvHeads * a.group + head : nullptr;
-                bool odd = false;
+            // A row that saw no key has weights of 2^-126 from Exp2Poly: it is known by its reference.
+            const float scale = top != -INFINITY || sum != sum ? 1.0f / sum : 0.0f;
+            const int head = w.h0 + row % p.pack;
+            const size_t at = (size_t)w.q0 + token;
+            T *out = (T *)a.out + at * a.outStride[0] + (size_t)head * a.outStride[1];
+            bool odd = false;
 #pragma unroll
-                for (int c = 0; c < D; c += 32) {
-                    float o[32];
-                    if (n > 0) {
-                        TmemLd32Issue(oAt + c, o);
-                        TmemLdWait32(o);
-                    } else {
+            for (int c = 0; c < D; c += 32) {
+                float o[32];
 #pragma unroll
-                        for (int e = 0; e < 32; e++) {
-                            o[e] = 0;
+                for (int e = 0; e < 32; e++) {
+                    o[e] = 0;
+                }
+                if (w.n > 0) {
+                    TmemLd32Issue(oAt + c, o);
+                    TmemLdWait32(o);
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                    odd |= !(fabsf(o[e]) <= 3.4e38f);
+                }
+                if (valid) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 16) {
+                        uint32_t pk[8];
+#pragma unroll
+                        for (int f = 0; f < 8; f++) {
+                            pk[f] = Pack2<T>(o[e + 2 * f] * scale, o[e + 2 * f + 1] * scale);
+                        }
+                        if (p.wide) {
+                            StGlobal32B(out + c + e, pk);
+                        } else {
+                            *(uint4 *)(out + c + e) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                            *(uint4 *)(out + c + e + 8) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
                         }
                     }
-#pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        odd |= !(fabsf(o[e]) <= 3.4e38f);
-                    }
-                    if (token < rows) {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            *(uint4 *)(out + c + e) = make_uint4(Pack2<T>(o[e] * scale, o[e + 1] * scale), Pack2<T>(o[e + 2] * scale, o[e + 3] * scale),
-                                                                 Pack2<T>(o[e + 4] * scale, o[e + 5] * scale), Pack2<T>(o[e + 6] * scale, o[e + 7] * scale));
-                        }
-                    }
                 }
-                if (lse != nullptr && token < rows) {
-                    *lse = top * factor * kLn2 + logf(sum);
-                }
-                unsigned again = __ballot_sync(~0u, odd && token < rows);
-                while (again != 0) {
-                    const int r = (warp & 3) * 32 + __ffs(again) - 1, t = t0 + i * half + r / p.pack, h = h0 + r % p.pack;
-                    again &= again - 1;
-                    const size_t q = (size_t)(q0 + t);
-                    AttendRow<T, D>((const T *)a.q + q * a.qStride[0] + (size_t)h * a.qStride[1], (const T *)a.k + (size_t)k0 * a.kStride[0] + (size_t)kvh * a.kStride[1],
-                                    a.kStride[0], (const T *)a.v + (size_t)k0 * a.vStride[0] + (size_t)kvh * a.vStride[1], a.vStride[0],
-                                    a.causal ? min(keys, t + past + 1) : keys, factor, (T *)a.out + q * a.outStride[0] + (size_t)h * a.outStride[1],
-                                    a.lse != nullptr ? a.lse + q * a.kvHeads * a.group + h : nullptr);
-                }
+            }
+            if (a.lse != nullptr && valid) {
+                a.lse[at * a.kvHeads * a.group + head] = top == -INFINITY ? -INFINITY : top * factor * kLn2 + logf(sum);
+            }
+            unsigned again = __ballot_sync(~0u, odd && valid);
+            while (again != 0) {
+                const int r = (warp & 3) * 32 + __ffs(again) - 1, t = w.t0 + i * half + r / p.pack, h = w.h0 + r % p.pack;
+                again &= again - 1;
+                const size_t q = (size_t)(w.q0 + t);
+                AttendRow<T, D>((const T *)a.q + q * a.qStride[0] + (size_t)h * a.qStride[1],
+                                (const T *)a.k + (size_t)w.k0 * a.kStride[0] + (size_t)w.kvh * a.kStride[1], a.kStride[0],
+                                (const T *)a.v + (size_t)w.k0 * a.vStride[0] + (size_t)w.kvh * a.vStride[1], a.vStride[0],
+                                a.causal ? min(w.keys, t + past + 1) : w.keys, factor, (T *)a.out + q * a.outStride[0] + (size_t)h * a.outStride[1],
+                                a.lse != nullptr ? a.lse + q * a.kvHeads * a.group + h : nullptr);
             }
         }
     }
@@ -411,15 +646,20 @@ int Launch(const mf_prefill_attention_args_t &a, cudaStream_t stream)
 {
     Params p;
     p.a = a;
-    p.pack = a.group & -a.group;
-    p.pack = p.pack > kTile ? kTile : p.pack;
-    p.tokens = 2 * kTile / p.pack;
+    // as many heads of a group as fill tiles of whole tokens to 15/16 at least, and divide the group
+    for (p.pack = a.group < kTile ? a.group : kTile; a.group % p.pack != 0 || kTile / p.pack * p.pack < kTile - kTile / 16; p.pack--) {
+    }
+    p.tokens = 2 * (kTile / p.pack);
+    p.wide = ((uintptr_t)a.out | (uint64_t)a.outStride[0] * sizeof(T) | (uint64_t)a.outStride[1] * sizeof(T)) % 32 == 0;
     p.headTiles = a.kvHeads * a.group / p.pack;
     p.tiles = a.tokensQ / p.tokens + a.B;
-    const long long ctas = (long long)p.tiles * p.headTiles;
-    if (ctas > 0x7fffffffll) {
-        return MF_K_TOO_LARGE;
+    const long long units = (long long)p.tiles * p.headTiles;
+    const int sms = mf_k_sm_count();
+    if (units > 0x7fffffffll || sms <= 0) {
+        return sms <= 0 ? MF_K_LAUNCH_FAILED : MF_K_TOO_LARGE;
     }
+    p.units = (int)units;
+    const unsigned ctas = units < sms ? (unsigned)units : (unsigned)sms;
     CUtensorMap q, k, v;
     constexpr bool kBf16 = Bf16<T>::value;
     // without keys their maps are never used, but have to describe something
@@ -431,7 +671,7 @@ int Launch(const mf_prefill_attention_args_t &a, cudaStream_t stream)
     }
     const size_t smem = sizeof(Shared<D>) + 1024;
     if (!mf::AllowSmem<mf_prefill_attention_kernel<T, D>>(smem) ||
-        LaunchDependent(mf_prefill_attention_kernel<T, D>, (unsigned)ctas, kThreads, smem, stream, q, k, v, p) != cudaSuccess) {
+        LaunchDependent(mf_prefill_attention_kernel<T, D>, ctas, kThreads, smem, stream, q, k, v, p) != cudaSuccess) {
         (void)cudaGetLastError();
         return MF_K_LAUNCH_FAILED;
     }
