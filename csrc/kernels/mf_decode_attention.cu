@@ -10,14 +10,18 @@
 // equal, contiguous piece of it, whichever rows that touches (lengths live on the device: the host sizes the grid only). A row that lies
 // within one CTA is written at once; of a row that crosses CTAs each leaves maximum, sum and unnormalised output in the workspace,
 // at most two per CTA, and a second kernel joins them in the order of the CTAs, so results do not depend on timing. Where no row has more
-// than kWholeTiles tiles, CTAs take whole rows and nothing has to be joined.
+// than kWholeKeys keys, CTAs take whole rows and nothing has to be joined.
 //
-// A CTA is four warps that share nothing but their position: each takes 16 keys of every tile, fetches them through its own ring of
-// cp.async stages (rows past the end of the sequence are filled with zeros: stale pages may hold anything, NaN included), computes
-// q k^T and p v with m16n8k16 products (the group's query heads are the 16 rows) and keeps its own running maximum and sum; they
-// meet at the end of a row. 8-bit caches are widened to fp16, which holds every e4m3 value; the query is scaled by a power of two per
-// head so that it fits fp16 without loss. p is rounded to the cache's type (fp16 for 8-bit caches) for the second product, as the
-// tensor cores want equal types; the sum is taken before that rounding, all sums in fp32.
+// A CTA is four warps that share nothing but their position: each takes a quarter of the keys of every tile, fetches them through its own ring
+// of cp.async stages (rows past the end of the sequence are filled with zeros: stale pages may hold anything, NaN included) and keeps its
+// own maximum and sum; they meet at the end of a row. Products are m16n8k16 with the keys (then the columns of v) as the 16 rows and eight
+// query heads as the columns, so a group of up to eight heads costs one product per 16 x 16 values of the cache and all statistics of a
+// head lie in the lanes that hold its results. The reference of the exponentials follows the maximum only where that has grown by more
+// than 2^8 (p stays below 256): most tiles need one vote for it, no shuffles and no scaling of the output.
+//
+// 8-bit caches are widened to fp16, which holds every e4m3 value; the query is scaled by a power of two per head so that it fits fp16
+// without loss. p is rounded to the cache's type (fp16 for 8-bit caches) for the second product, as the tensor cores want equal
+// types; the sum is taken before that rounding, all sums in fp32.
 #include "mf/device/mf_shm_device.cuh"
 #include "mf_attention.cuh"
 #include "mf_kernels.h"
@@ -30,22 +34,28 @@ using namespace mf::attn;
 using mf::sm100::GridDependency;
 
 constexpr int kThreads = 128;
+constexpr int kCtasPerSm = 2;
 constexpr int kWarps = 4;
-constexpr int kWarpKeys = 16;
-constexpr int kTileKeys = kWarps * kWarpKeys;
-constexpr int kWholeTiles = 4;
-constexpr int kRows = 16;                  // query heads of a tile
-constexpr uint32_t kWarpRing = 24 * 1024;  // bytes of a warp's stages
-constexpr int kPartialFloats = 2;          // maximum and sum before a row's values
+constexpr int kWholeKeys = 256;
+constexpr int kRowCost = 3;        // tiles that beginning and ending a row takes as long as
+constexpr int kPartialFloats = 2;  // maximum and sum before a row's values
+constexpr int kLeastPiece = 2;
+constexpr int kJoinGroups = 4;     // of threads that share the parts of a row in the second kernel
+constexpr float kSlack = 8.0f;     // powers of two by which the reference may lag behind the maximum
 
-template <typename C, int D>
+template <typename C, int D, int NT>
 struct Cfg {
     static constexpr uint32_t kRow = D * sizeof(C);
     static constexpr uint32_t kChunks = kRow / 16;
-    static constexpr uint32_t kStage = kWarpKeys * kRow * 2;
-    static constexpr int kStages = kWarpRing / kStage > 8 ? 8 : kWarpRing / kStage;
+    static constexpr int kBlocks = kRow <= 128 ? 2 : 1;  // of 16 keys: narrow rows are worked on two by two
+    static constexpr int kWarpKeys = 16 * kBlocks, kTileKeys = kWarps * kWarpKeys, kWholeTiles = kWholeKeys / kTileKeys;
+    static constexpr uint32_t kStage = kWarpKeys * kRow * 2;  // keys and values of a warp's part of a tile
+    static constexpr int kStages = 24576 / kStage;
     static constexpr uint32_t kRing = kStages * kStage;
-    static constexpr uint32_t kSmem = kWarps * kRing + kRows * D * 4;
+    static constexpr int kRows = 8 * NT;
+    static constexpr int kJoinRow = D + 4;  // floats from head to head: the lanes of a store fall into 32 banks
+    static constexpr int kJoins = 2 / NT;   // buffers in which the warps add up a row
+    static constexpr uint32_t kSmem = kWarps * kRing + kJoins * kRows * kJoinRow * 4;
     static __device__ __forceinline__ uint32_t Place(uint32_t row, uint32_t chunk)
     {
         const uint32_t x = kRow >= 128 ? row & 7 : (row >> 1) & 3;  // eight rows of one chunk lie in eight different bank groups
@@ -58,10 +68,12 @@ struct Cursor {
     int b, hg, tile, tiles, length;
 };
 
+template <int TILE>
 struct Line {
     const int *lengths;
     const int *rows;
     int B, HG, cap, tableRows;
+    static __device__ __forceinline__ int Tiles(int length) { return (length + TILE - 1) / TILE; }
     __device__ __forceinline__ int Seq(int b) const { return rows != nullptr ? rows[b] : b; }
     __device__ __forceinline__ int Length(int b) const
     {
@@ -79,7 +91,7 @@ struct Line {
             }
         }
         c.b = b;
-        c.tiles = (c.length + kTileKeys - 1) / kTileKeys;
+        c.tiles = Tiles(c.length);
     }
     __device__ __forceinline__ void Next(Cursor &c) const
     {
@@ -102,23 +114,25 @@ struct Operand<Q, __nv_fp8_e4m3> {
     using type = __half;
 };
 
-// One partial result: [row]{maximum, sum} of kRows rows, then [row][D] values. Two per CTA: of the row that it enters in the middle, and of
+// One partial result: [row]{reference, sum} of ROWS rows, then [row][D] values. Two per CTA: of the row that it enters in the middle, and of
 // the row that goes on behind it.
-template <int D>
+template <int D, int ROWS>
 __device__ __forceinline__ float *Partial(float *ws, int cta, int which)
 {
-    return ws + ((size_t)cta * 2 + which) * (kRows * (D + kPartialFloats));
+    return ws + ((size_t)cta * 2 + which) * (ROWS * (D + kPartialFloats));
 }
 
-template <typename Q, typename C, int D>
-__global__ void __launch_bounds__(kThreads, 2) mf_decode_attention_kernel(const __grid_constant__ mf_decode_attention_args_t a)
+// NT: query heads of a row of the line, in eights.
+template <typename Q, typename C, int D, int NT>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) mf_decode_attention_kernel(const __grid_constant__ mf_decode_attention_args_t a)
 {
-    using X = Cfg<C, D>;
+    using X = Cfg<C, D, NT>;
     using T = typename Operand<Q, C>::type;
     constexpr bool kWide = sizeof(C) == 1;
-    constexpr int kSteps = D / 16;  // products along D of q k^T; pairs of column tiles of p v
+    using L = Line<X::kTileKeys>;
+    constexpr int kRows = X::kRows, kSteps = D / 16, kBlocks = X::kBlocks, kWarpKeys = X::kWarpKeys, kTileKeys = X::kTileKeys;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ float joinMax[kWarps][kRows], joinSum[kWarps][kRows];
+    __shared__ float joinTop[kWarps][kRows], joinSum[kWarps][kRows];
     __shared__ long long scan[kWarps][2];
     __shared__ int scanMax[kWarps];
     __shared__ int startB;
@@ -127,15 +141,15 @@ __global__ void __launch_bounds__(kThreads, 2) mf_decode_attention_kernel(const 
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = lane >> 2, pos = lane & 3;
     const int GT = (a.group + kRows - 1) / kRows, HG = a.kvHeads * GT;
-    const Line line{a.lengths, a.rows, a.B, HG, a.tableWidth * a.pageSize, a.tableRows};
+    const L line{a.lengths, a.rows, a.B, HG, a.tableWidth * a.pageSize, a.tableRows};
 
     // ---- where this CTA's piece of the line begins and how long it is
     const int per = (a.B + kThreads - 1) / kThreads, b0 = min(a.B, tid * per), b1 = min(a.B, b0 + per);
     long long tiles = 0, rows = 0;
     int longest = 0;
     for (int b = b0; b < b1; b++) {
-        const int n = (line.Length(b) + kTileKeys - 1) / kTileKeys;
-        tiles += n;
+        const int n = L::Tiles(line.Length(b));
+        tiles += n > 0 ? n + kRowCost : 0;
         rows += n > 0;
         longest = max(longest, n);
     }
@@ -169,21 +183,24 @@ __global__ void __launch_bounds__(kThreads, 2) mf_decode_attention_kernel(const 
         }
         longest = max(longest, scanMax[w]);
     }
-    const bool whole = longest <= kWholeTiles;
-    const long long units = (whole ? total[1] : total[0]) * HG;
-    // a piece is worth a CTA from kWholeTiles tiles on; the CTAs behind the last piece have none
-    const long long wanted = whole ? units : (units + kWholeTiles - 1) / kWholeTiles, parts = wanted < gridDim.x ? wanted : gridDim.x;
-    long long first = 0, left = 0;
+    const bool whole = longest <= X::kWholeTiles;
+    // The line in units: a row is kRowCost of them, then one for each tile; or one if rows are not cut. A piece is worth a CTA from
+    // kLeastPiece units on; the CTAs behind the last piece have none.
+    const int price = whole ? 1 : kRowCost;
+    const long long units = (whole ? total[1] : total[0]) * HG, wanted = whole ? units : (units + kLeastPiece - 1) / kLeastPiece,
+                    parts = wanted < gridDim.x ? wanted : gridDim.x;
+    long long first = 0, last = 0;
     if (blockIdx.x < parts) {
         first = units * blockIdx.x / parts;
-        left = units * (blockIdx.x + 1) / parts - first;
+        last = units * (blockIdx.x + 1) / parts;
     }
     {
-        long long at = (whole ? before[1] : before[0]) * HG, mine = (whole ? rows : tiles) * HG;
-        if (left > 0 && first >= at && first < at + mine) {
+        long long at = (whole ? before[1] : before[0]) * HG;
+        const long long mine = (whole ? rows : tiles) * HG;
+        if (first < last && first >= at && first < at + mine) {
             for (int b = b0; b < b1; b++) {
-                const int n = (line.Length(b) + kTileKeys - 1) / kTileKeys;
-                const long long here = (long long)(whole ? n > 0 : n) * HG;
+                const int n = L::Tiles(line.Length(b));
+                const long long here = (long long)(n == 0 ? 0 : whole ? 1 : n + price) * HG;
                 if (first < at + here) {
                     startB = b;
                     startOff = first - at;
@@ -212,37 +229,48 @@ __global__ void __launch_bounds__(kThreads, 2) mf_decode_attention_kernel(const 
     if (tid < 2 && a.workspace != nullptr) {
         ((int2 *)a.marks)[blockIdx.x * 2 + tid] = make_int2(-1, -1);  // {sequence, head group} of the two partial results
     }
-    if (left <= 0) {
+    if (first >= last) {
         return;
     }
+    // A CTA that begins within a row's cost begins with its first tile; one that ends there leaves the row to the next CTA. `left`: units from
+    // the current tile's to the piece's end, none if not above 0.
     Cursor cur;
     line.Open(cur, startB);
-    if (whole) {
-        cur.hg = (int)startOff;
-        cur.tile = 0;
-    } else {
-        cur.hg = (int)(startOff / cur.tiles);
-        cur.tile = (int)(startOff % cur.tiles);
-    }
+    const int all = whole ? 1 : price + cur.tiles, into = (int)(startOff % all);
+    cur.hg = (int)(startOff / all);
+    cur.tile = into > price ? into - price : 0;
+    long long left = last - first - (whole || into > price ? 0 : price - into);
+    auto next = [&](Cursor &c, long long &units) {
+        const bool end = c.tile + 1 == c.tiles;
+        units -= whole ? end : end ? 1 + price : 1;
+        line.Next(c);
+    };
 
     // ---- the warp's ring of stages
     const uint32_t ring = SmemAddr32(smem) + warp * X::kRing;
     float *join = (float *)(smem + kWarps * X::kRing);
+    const bool together = a.pageSize % 16 == 0;  // 16 keys from a multiple of 16 on lie in one page
     Cursor ahead = cur;
     long long aheadLeft = left;
     uint32_t fill = 0;
     auto fetch = [&]() {
         if (aheadLeft > 0) {
-            const int key0 = ahead.tile * kTileKeys + warp * kWarpKeys;
-            if (key0 < ahead.length) {
-                // each lane looks one of the 16 rows up
-                const int key = key0 + (lane & 15);
-                const uint32_t page = (uint32_t)key / (uint32_t)a.pageSize, slot = (uint32_t)key % (uint32_t)a.pageSize;
-                long long off = -1;
+            const int *entry = a.table + (size_t)line.Seq(ahead.b) * a.tableStride;
+            const long long head = (ahead.hg / GT) * a.stride[1];
+#pragma unroll
+            for (int block = 0; block < kBlocks; block++) {
+                const int key0 = ahead.tile * kTileKeys + warp * kWarpKeys + block * 16;
+                if (key0 >= ahead.length) {
+                    break;
+                }
+                // each lane looks the first or one of the 16 rows up: its offset in elements, or -1
+                const int key = key0 + (together ? 0 : lane & 15);
+                long long own = -1;
                 if (key < ahead.length) {
-                    const int p = a.table[(size_t)line.Seq(ahead.b) * a.tableStride + page];
+                    const uint32_t page = a.pageSize == 1 ? key : __umulhi((uint32_t)key, a.pageMagic) >> a.pageShift;
+                    const int p = entry[page];
                     if (p >= 0 && p < a.pages) {
-                        off = p * a.stride[0] + (ahead.hg / GT) * a.stride[1] + (long long)slot * a.stride[2];
+                        own = p * a.stride[0] + head + (long long)((uint32_t)key - page * (uint32_t)a.pageSize) * a.stride[2];
                     } else if (a.status != nullptr) {
                         *a.status = MF_DEV_ERR_BOUNDS;
                     }
@@ -250,17 +278,17 @@ __global__ void __launch_bounds__(kThreads, 2) mf_decode_attention_kernel(const 
                 const uint32_t at = ring + fill * X::kStage;
                 constexpr int kPer = 32 / X::kChunks;  // rows of one trip
 #pragma unroll
-                for (int i = 0; i < kWarpKeys / kPer; i++) {
+                for (int i = 0; i < 16 / kPer; i++) {
                     const uint32_t row = i * kPer + lane / X::kChunks, chunk = lane % X::kChunks;
-                    const long long o = __shfl_sync(~0u, off, row);
-                    const uint32_t bytes = o >= 0 ? 16 : 0;
-                    const size_t from = o >= 0 ? (size_t)o * sizeof(C) + chunk * 16 : 0;
-                    CpAsync16(at + X::Place(row, chunk), (const unsigned char *)a.k + from, bytes);
-                    CpAsync16(at + kWarpKeys * X::kRow + X::Place(row, chunk), (const unsigned char *)a.v + from, bytes);
+                    const long long o = together ? own : __shfl_sync(~0u, own, row);
+                    const bool there = o >= 0 && key0 + (int)row < ahead.length;
+                    const size_t from = there ? (size_t)(o + (together ? row * a.stride[2] : 0)) * sizeof(C) + chunk * 16 : 0;
+                    const uint32_t to = at + X::Place(block * 16 + row, chunk);
+                    CpAsync16(to, (const unsigned char *)a.k + from, there ? 16 : 0);
+                    CpAsync16(to + kWarpKeys * X::kRow, (const unsigned char *)a.v + from, there ? 16 : 0);
                 }
             }
-            aheadLeft -= !whole || ahead.tile + 1 == ahead.tiles;
-            line.Next(ahead);
+            next(ahead, aheadLeft);
         }
         CpCommit();
         fill = fill + 1 == X::kStages ? 0 : fill + 1;
@@ -270,233 +298,313 @@ __global__ void __launch_bounds__(kThreads, 2) mf_decode_attention_kernel(const 
         fetch();
     }
 
-    uint32_t q[kSteps][4];
-    float acc[D / 8][4];
-    float top[2], sum[2], factor[2];
+    uint32_t q[NT][kSteps][2];
+    float acc[NT][kSteps][4];  // 16 columns of v by 8 heads each
+    float top[NT][2], sum[NT][2], factor[NT][2];  // of the two heads whose results the lane holds
+    float ks = 1.0f;
+    // A row's query heads, lane by lane as the products want them. 8-bit keys come as four neighbouring columns to a lane, 16-bit ones as two and two.
+    auto loadQueries = [&](const Cursor &c) {
+        const int kvh = c.hg / GT, g0 = (c.hg % GT) * kRows;
+        if (kWide) {
+            ks = a.kScale[kvh];
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const int g = g0 + t * 8 + quad;
+            const Q *src = (const Q *)a.q + (size_t)c.b * a.qStride[0] + (size_t)(kvh * a.group + g) * a.qStride[1];
+#pragma unroll
+            for (int s = 0; s < kSteps; s++) {
+                const int d = s * 16 + (kWide ? pos * 4 : pos * 2);
+                q[t][s][0] = g < a.group ? *(const uint32_t *)(src + d) : 0;
+                q[t][s][1] = g < a.group ? *(const uint32_t *)(src + d + (kWide ? 2 : 8)) : 0;
+            }
+        }
+    };
+    loadQueries(cur);
     uint32_t take = 0;
     int rowStart = 0;
     bool open = true;
     while (left > 0) {
-        if (open) {  // a row begins: its query heads, lane by lane as the products want them
+        if (open) {  // a row begins
             open = false;
             rowStart = cur.tile;
-            const int kvh = cur.hg / GT, g0 = (cur.hg % GT) * kRows;
-            const float ks = kWide ? a.kScale[kvh] : 1.0f;
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                const int g = g0 + quad + half * 8;
-                const Q *src = (const Q *)a.q + (size_t)cur.b * a.qStride[0] + (size_t)(kvh * a.group + g) * a.qStride[1];
-                float biggest = 0;
+            for (int t = 0; t < NT; t++) {
+                float up = 1.0f;
+                if (kWide) {
+                    float biggest = 0;
 #pragma unroll
-                for (int s = 0; s < kSteps; s++) {
-                    // 8-bit keys come as four neighbouring columns to a lane, 16-bit ones as two and two
-                    const int d = s * 16 + (kWide ? pos * 4 : pos * 2);
-                    uint32_t lo = 0, hi = 0;
-                    if (g < a.group) {
-                        lo = *(const uint32_t *)(src + d);
-                        hi = *(const uint32_t *)(src + d + (kWide ? 2 : 8));
-                    }
-                    q[s][half] = lo;
-                    q[s][half + 2] = hi;
-                    if (kWide) {
-                        const float2 x = Unpack2<Q>(lo), y = Unpack2<Q>(hi);
+                    for (int s = 0; s < kSteps; s++) {
+                        const float2 x = Unpack2<Q>(q[t][s][0]), y = Unpack2<Q>(q[t][s][1]);
                         biggest = fmaxf(fmaxf(biggest, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(y.x), fabsf(y.y)));
                     }
-                }
-                factor[half] = a.scale * kLog2e * ks;
-                if (kWide) {
                     biggest = fmaxf(biggest, __shfl_xor_sync(~0u, biggest, 1));
                     biggest = fmaxf(biggest, __shfl_xor_sync(~0u, biggest, 2));
                     int e = (int)(__float_as_uint(biggest) >> 23) - 127;  // its exponent: scaled values lie below two
                     e = biggest == 0 || e > 126 ? 0 : e < -100 ? -100 : e;
                     const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                    factor[half] *= __uint_as_float((uint32_t)(127 + e) << 23);
+                    up = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
                     for (int s = 0; s < kSteps; s++) {
-                        const float2 x = Unpack2<Q>(q[s][half]), y = Unpack2<Q>(q[s][half + 2]);
-                        q[s][half] = Pack2<__half>(x.x * down, x.y * down);
-                        q[s][half + 2] = Pack2<__half>(y.x * down, y.y * down);
+                        const float2 x = Unpack2<Q>(q[t][s][0]), y = Unpack2<Q>(q[t][s][1]);
+                        q[t][s][0] = Pack2<__half>(x.x * down, x.y * down);
+                        q[t][s][1] = Pack2<__half>(y.x * down, y.y * down);
                     }
                 }
-                top[half] = -INFINITY;
-                sum[half] = 0;
-            }
 #pragma unroll
-            for (int n = 0; n < D / 8; n++) {
-                acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0;
+                for (int e = 0; e < 2; e++) {
+                    factor[t][e] = a.scale * kLog2e * ks * (kWide ? __shfl_sync(~0u, up, (2 * pos + e) * 4) : 1.0f);
+                    top[t][e] = -INFINITY;
+                    sum[t][e] = 0;
+                }
+#pragma unroll
+                for (int s = 0; s < kSteps; s++) {
+                    acc[t][s][0] = acc[t][s][1] = acc[t][s][2] = acc[t][s][3] = 0;
+                }
             }
         }
         CpWait<X::kStages - 2>();
         __syncwarp();  // the stage is there for all lanes, and nobody reads the one before it any more: that one is filled again
         fetch();
         const int key0 = cur.tile * kTileKeys + warp * kWarpKeys;
+        const uint32_t at = ring + take * X::kStage;
         if (key0 < cur.length) {
-            const uint32_t at = ring + take * X::kStage;
-            float s0[4] = {0, 0, 0, 0}, s1[4] = {0, 0, 0, 0};
-            const uint32_t kRowOf = (lane & 7) + ((lane >> 4) << 3), kChunkOf = (lane >> 3) & 1;
-            if (kWide) {
+            // A block behind the end of the sequence holds what was there before: its scores are masked, its values left alone.
+            const int blocks = kBlocks == 1 || key0 + 16 >= cur.length ? 1 : kBlocks;
+            float x[kBlocks][NT][4];  // [key quad, quad + 8][head 2 pos, 2 pos + 1]
+            bool grown = false;
 #pragma unroll
-                for (int s = 0; s < kSteps; s += 2) {
-                    uint32_t m[4];
-                    LdMatrix4(m, at + X::Place(kRowOf, s + kChunkOf));
-                    Mma16x8x16<T>(s0, q[s], E4m3ToHalf2(m[0]), E4m3ToHalf2(m[0] >> 16));
-                    Mma16x8x16<T>(s1, q[s], E4m3ToHalf2(m[2]), E4m3ToHalf2(m[2] >> 16));
-                    Mma16x8x16<T>(s0, q[s + 1], E4m3ToHalf2(m[1]), E4m3ToHalf2(m[1] >> 16));
-                    Mma16x8x16<T>(s1, q[s + 1], E4m3ToHalf2(m[3]), E4m3ToHalf2(m[3] >> 16));
+            for (int block = 0; block < kBlocks; block++) {
+                float y[2][NT][4];  // two chains of products
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        y[0][t][e] = y[1][t][e] = 0;
+                    }
                 }
-            } else {
+                if (kWide) {
+                    // matrices: keys 0-7 and 8-15 of one chunk, the same of the next; four neighbouring columns to a lane
 #pragma unroll
-                for (int s = 0; s < kSteps; s++) {
-                    uint32_t m[4];
-                    LdMatrix4(m, at + X::Place(kRowOf, 2 * s + kChunkOf));
-                    Mma16x8x16<T>(s0, q[s], m[0], m[1]);
-                    Mma16x8x16<T>(s1, q[s], m[2], m[3]);
-                }
-            }
-            uint32_t p[4];
+                    for (int s = 0; s < kSteps; s += 2) {
+                        uint32_t m[4];
+                        LdMatrix4(m, at + X::Place(block * 16 + (lane & 15), s + (lane >> 4)));
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                float x[4] = {s0[2 * half] * factor[half], s0[2 * half + 1] * factor[half], s1[2 * half] * factor[half], s1[2 * half + 1] * factor[half]};
-                if (key0 + kWarpKeys > cur.length) {
+                        for (int c = 0; c < 2; c++) {
+                            const uint32_t a0 = E4m3ToHalf2(m[2 * c]), a1 = E4m3ToHalf2(m[2 * c + 1]), a2 = E4m3ToHalf2(m[2 * c] >> 16),
+                                           a3 = E4m3ToHalf2(m[2 * c + 1] >> 16);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if (key0 + (i >> 1) * 8 + pos * 2 + (i & 1) >= cur.length) {
-                            x[i] = -INFINITY;
+                            for (int t = 0; t < NT; t++) {
+                                Mma16x8x16<T>(y[c][t], a0, a1, a2, a3, q[t][s + c][0], q[t][s + c][1]);
+                            }
+                        }
+                    }
+                } else {
+                    // matrices: keys 0-7 and 8-15 of the first eight columns, the same of the next eight
+#pragma unroll
+                    for (int s = 0; s < kSteps; s++) {
+                        uint32_t m[4];
+                        LdMatrix4(m, at + X::Place(block * 16 + (lane & 15), 2 * s + (lane >> 4)));
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            Mma16x8x16<T>(y[s & 1][t], m[0], m[1], m[2], m[3], q[t][s][0], q[t][s][1]);
                         }
                     }
                 }
-                float best = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                best = fmaxf(best, __shfl_xor_sync(~0u, best, 1));
-                best = fmaxf(best, __shfl_xor_sync(~0u, best, 2));
-                best = fmaxf(best, top[half]);
-                const float base = best == -INFINITY ? 0.0f : best, shrink = Exp2(top[half] - base);
-                top[half] = best;
-                float add = 0;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    x[i] = Exp2(x[i] - base);
-                    add += x[i];
-                }
-                sum[half] = sum[half] * shrink + add;  // of this lane's columns; the four lanes of a row are added at its end
+                for (int t = 0; t < NT; t++) {
 #pragma unroll
-                for (int n = 0; n < D / 8; n++) {
-                    acc[n][2 * half] *= shrink;
-                    acc[n][2 * half + 1] *= shrink;
-                }
-                p[half] = Pack2<T>(x[0], x[1]);
-                p[half + 2] = Pack2<T>(x[2], x[3]);
-            }
-            const uint32_t vAt = at + kWarpKeys * X::kRow, vRowOf = lane & 15, vChunkOf = lane >> 4;
-            if (kWide) {
-#pragma unroll
-                for (int s = 0; s < kSteps; s += 2) {
-                    uint32_t m[4];
-                    LdMatrix4T(m, vAt + X::Place(vRowOf, s + vChunkOf));
-#pragma unroll
-                    for (int c = 0; c < 2; c++) {  // a 16-bit unit holds an even and an odd column of one key: they go to two column tiles
-                        Mma16x8x16<T>(acc[2 * (s + c)], p, E4m3ToHalf2(__byte_perm(m[2 * c], 0, 0x4420)), E4m3ToHalf2(__byte_perm(m[2 * c + 1], 0, 0x4420)));
-                        Mma16x8x16<T>(acc[2 * (s + c) + 1], p, E4m3ToHalf2(__byte_perm(m[2 * c], 0, 0x4431)),
-                                      E4m3ToHalf2(__byte_perm(m[2 * c + 1], 0, 0x4431)));
+                    for (int e = 0; e < 4; e++) {
+                        const bool seen = key0 + block * 16 + quad + (e >> 1) * 8 < cur.length;
+                        x[block][t][e] = seen ? (y[0][t][e] + y[1][t][e]) * factor[t][e & 1] : -INFINITY;
+                        grown |= x[block][t][e] - top[t][e & 1] > kSlack;
                     }
                 }
-            } else {
+            }
+            if (__any_sync(~0u, grown)) {
 #pragma unroll
-                for (int s = 0; s < kSteps; s++) {
-                    uint32_t m[4];
-                    LdMatrix4T(m, vAt + X::Place(vRowOf, 2 * s + vChunkOf));
-                    Mma16x8x16<T>(acc[2 * s], p, m[0], m[1]);
-                    Mma16x8x16<T>(acc[2 * s + 1], p, m[2], m[3]);
+                for (int t = 0; t < NT; t++) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float best = top[t][e];
+#pragma unroll
+                        for (int block = 0; block < kBlocks; block++) {
+                            best = fmaxf(best, fmaxf(x[block][t][e], x[block][t][e + 2]));
+                        }
+                        best = fmaxf(best, __shfl_xor_sync(~0u, best, 4));
+                        best = fmaxf(best, __shfl_xor_sync(~0u, best, 8));
+                        best = fmaxf(best, __shfl_xor_sync(~0u, best, 16));
+                        const float shrink = Exp2(top[t][e] - (best == -INFINITY ? 0.0f : best));
+                        top[t][e] = best;
+                        sum[t][e] *= shrink;
+#pragma unroll
+                        for (int s = 0; s < kSteps; s++) {
+                            acc[t][s][e] *= shrink;
+                            acc[t][s][e + 2] *= shrink;
+                        }
+                    }
+                }
+            }
+            const uint32_t vAt = at + kWarpKeys * X::kRow;
+#pragma unroll
+            for (int block = 0; block < kBlocks; block++) {
+                if (block >= blocks) {
+                    break;
+                }
+                uint32_t p[NT][2];
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float from = top[t][e & 1];
+                        x[block][t][e] = Exp2(x[block][t][e] - (from == -INFINITY ? 0.0f : from));
+                        sum[t][e & 1] += x[block][t][e];  // of this lane's keys; the lanes of a head are added at the end of the row
+                    }
+                    p[t][0] = Transposed8x8(Pack2<T>(x[block][t][0], x[block][t][1]));
+                    p[t][1] = Transposed8x8(Pack2<T>(x[block][t][2], x[block][t][3]));
+                }
+                if (kWide) {
+                    // matrices, transposed: keys 0-7 and 8-15 of a chunk, the same of the next. A 16-bit unit holds an even and an odd column of one key:
+                    // even columns are the first eight rows of the product, odd ones the others.
+#pragma unroll
+                    for (int s = 0; s < kSteps; s += 2) {
+                        uint32_t m[4];
+                        LdMatrix4T(m, vAt + X::Place(block * 16 + (lane & 15), s + (lane >> 4)));
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+                            const uint32_t lo = m[2 * c], hi = m[2 * c + 1];
+                            const uint32_t a0 = E4m3ToHalf2(__byte_perm(lo, 0, 0x4420)), a1 = E4m3ToHalf2(__byte_perm(lo, 0, 0x4431)),
+                                           a2 = E4m3ToHalf2(__byte_perm(hi, 0, 0x4420)), a3 = E4m3ToHalf2(__byte_perm(hi, 0, 0x4431));
+#pragma unroll
+                            for (int t = 0; t < NT; t++) {
+                                Mma16x8x16<T>(acc[t][s + c], a0, a1, a2, a3, p[t][0], p[t][1]);
+                            }
+                        }
+                    }
+                } else {
+                    // matrices, transposed: columns 0-7 and 8-15 of keys 0-7, the same of keys 8-15
+#pragma unroll
+                    for (int s = 0; s < kSteps; s++) {
+                        uint32_t m[4];
+                        LdMatrix4T(m, vAt + X::Place(block * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * s + ((lane >> 3) & 1)));
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            Mma16x8x16<T>(acc[t][s], m[0], m[1], m[2], m[3], p[t][0], p[t][1]);
+                        }
+                    }
                 }
             }
         }
         take = take + 1 == X::kStages ? 0 : take + 1;
-        left -= !whole || cur.tile + 1 == cur.tiles;
+        const Cursor done = cur;
         const bool rowEnd = cur.tile + 1 == cur.tiles;
+        next(cur, left);
         if (rowEnd || left <= 0) {
+            if (left > 0) {
+                loadQueries(cur);  // on their way while the row is put together
+            }
             // ---- the four warps' results of this row become one
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                sum[half] += __shfl_xor_sync(~0u, sum[half], 1);
-                sum[half] += __shfl_xor_sync(~0u, sum[half], 2);
-                if (pos == 0) {
-                    joinMax[warp][quad + half * 8] = top[half];
-                    joinSum[warp][quad + half * 8] = sum[half];
+            for (int t = 0; t < NT; t++) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    sum[t][e] += __shfl_xor_sync(~0u, sum[t][e], 4);
+                    sum[t][e] += __shfl_xor_sync(~0u, sum[t][e], 8);
+                    sum[t][e] += __shfl_xor_sync(~0u, sum[t][e], 16);
+                    if (quad == 0) {
+                        joinTop[warp][t * 8 + 2 * pos + e] = top[t][e];
+                        joinSum[warp][t * 8 + 2 * pos + e] = sum[t][e];
+                    }
                 }
             }
             __syncthreads();
-            float weight[2];
+            float weight[NT][2];
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                const int r = quad + half * 8;
-                const float best = fmaxf(fmaxf(joinMax[0][r], joinMax[1][r]), fmaxf(joinMax[2][r], joinMax[3][r]));
-                weight[half] = best == -INFINITY ? 0.0f : Exp2(top[half] - best);
+            for (int t = 0; t < NT; t++) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int r = t * 8 + 2 * pos + e;
+                    const float best = fmaxf(fmaxf(joinTop[0][r], joinTop[1][r]), fmaxf(joinTop[2][r], joinTop[3][r]));
+                    weight[t][e] = best == -INFINITY ? 0.0f : Exp2(top[t][e] - best);
+                }
             }
-            // a quarter of the columns at a time, each warp at another one: the order of the additions is fixed by the quarter
+            // A part of the columns at a time, each warp that adds up in the same buffer at another one: the order of the additions is fixed.
+            constexpr int kTurns = kWarps / X::kJoins;
+            float *mine = join + warp / kTurns * (kRows * X::kJoinRow);
 #pragma unroll
-            for (int turn = 0; turn < kWarps; turn++) {
-                const int part = (warp + turn) & 3;
+            for (int turn = 0; turn < kTurns; turn++) {
+                const int part = (warp + turn) % kTurns;
 #pragma unroll
-                for (int n = 0; n < D / 8; n++) {
-                    if (n / (D / 32) == part) {
+                for (int s = 0; s < kSteps; s++) {
+                    if (s / (kSteps / kTurns) == part) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const int col = kWide ? (n >> 1) * 16 + pos * 4 + (e & 1) * 2 + (n & 1) : n * 8 + pos * 2 + (e & 1);
-                            float *at = join + (quad + (e >> 1) * 8) * D + col;
-                            const float x = acc[n][e] * weight[e >> 1];
-                            *at = turn == 0 ? x : *at + x;
+                        for (int t = 0; t < NT; t++) {
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const int d = s * 16 + (kWide ? 2 * quad + (e >> 1) : quad + (e >> 1) * 8);
+                                float *place = mine + (t * 8 + 2 * pos + (e & 1)) * X::kJoinRow + d;
+                                const float y = acc[t][s][e] * weight[t][e & 1];
+                                *place = turn == 0 ? y : *place + y;
+                            }
                         }
                     }
                 }
                 __syncthreads();
             }
-            const int kvh = cur.hg / GT, g0 = (cur.hg % GT) * kRows;
+            const int kvh = done.hg / GT, g0 = (done.hg % GT) * kRows;
             const bool complete = rowEnd && rowStart == 0;
             const int which = rowStart != 0 ? 0 : 1;
             const float vs = kWide ? a.vScale[kvh] : 1.0f;
             for (int i = tid; i < kRows * (D / 8); i += kThreads) {
                 const int r = i / (D / 8), d = (i % (D / 8)) * 8;
-                const float best = fmaxf(fmaxf(joinMax[0][r], joinMax[1][r]), fmaxf(joinMax[2][r], joinMax[3][r]));
+                const float best = fmaxf(fmaxf(joinTop[0][r], joinTop[1][r]), fmaxf(joinTop[2][r], joinTop[3][r]));
                 float all = 0;
 #pragma unroll
                 for (int w = 0; w < kWarps; w++) {
-                    all += best == -INFINITY ? 0.0f : joinSum[w][r] * Exp2(joinMax[w][r] - best);
+                    all += best == -INFINITY ? joinSum[w][r] : joinSum[w][r] * Exp2(joinTop[w][r] - best);
                 }
-                const float4 x = *(const float4 *)(join + r * D + d), y = *(const float4 *)(join + r * D + d + 4);
+                float4 y = *(const float4 *)(join + r * X::kJoinRow + d), z = *(const float4 *)(join + r * X::kJoinRow + d + 4);
+                if (X::kJoins == 2) {
+                    const float *other = join + kRows * X::kJoinRow + r * X::kJoinRow + d;
+                    const float4 y1 = *(const float4 *)other, z1 = *(const float4 *)(other + 4);
+                    y = make_float4(y.x + y1.x, y.y + y1.y, y.z + y1.z, y.w + y1.w);
+                    z = make_float4(z.x + z1.x, z.y + z1.y, z.z + z1.z, z.w + z1.w);
+                }
                 if (!complete) {
-                    float *ws = Partial<D>((float *)a.workspace, blockIdx.x, which);
+                    float *ws = Partial<D, kRows>((float *)a.workspace, blockIdx.x, which);
                     if (d == 0) {
                         *(float2 *)(ws + r * kPartialFloats) = make_float2(best, all);
                     }
                     ws += kRows * kPartialFloats + r * D + d;
-                    *(float4 *)ws = x;
-                    *(float4 *)(ws + 4) = y;
+                    *(float4 *)ws = y;
+                    *(float4 *)(ws + 4) = z;
                 } else if (g0 + r < a.group) {
                     const int h = kvh * a.group + g0 + r;
                     const float scale = (all != 0 ? 1.0f / all : 0.0f) * vs;
-                    uint4 packed = make_uint4(Pack2<Q>(x.x * scale, x.y * scale), Pack2<Q>(x.z * scale, x.w * scale), Pack2<Q>(y.x * scale, y.y * scale),
-                                              Pack2<Q>(y.z * scale, y.w * scale));
-                    *(uint4 *)((Q *)a.out + (size_t)cur.b * a.outStride[0] + (size_t)h * a.outStride[1] + d) = packed;
+                    uint4 packed = make_uint4(Pack2<Q>(y.x * scale, y.y * scale), Pack2<Q>(y.z * scale, y.w * scale), Pack2<Q>(z.x * scale, z.y * scale),
+                                              Pack2<Q>(z.z * scale, z.w * scale));
+                    *(uint4 *)((Q *)a.out + (size_t)done.b * a.outStride[0] + (size_t)h * a.outStride[1] + d) = packed;
                     if (a.lse != nullptr && d == 0) {
-                        a.lse[(size_t)cur.b * a.kvHeads * a.group + h] = best * kLn2 + logf(all);
+                        a.lse[(size_t)done.b * a.kvHeads * a.group + h] = best * kLn2 + logf(all);
                     }
                 }
             }
             if (!complete && tid == 0) {
-                ((int2 *)a.marks)[blockIdx.x * 2 + which] = make_int2(cur.b, cur.hg);
+                ((int2 *)a.marks)[blockIdx.x * 2 + which] = make_int2(done.b, done.hg);
             }
             __syncthreads();
             open = true;
         }
-        line.Next(cur);
     }
     CpWait<0>();
 }
 
 // One CTA for each row that is continued behind CTA blockIdx.x of the first kernel: that one's second partial result and the first ones
 // of the CTAs behind it, as long as they are of the same row. A thread owns eight columns of a query head.
-template <typename Q, int D, bool WIDE>
-__global__ void __launch_bounds__(kRows * 16) mf_decode_join_kernel(const __grid_constant__ mf_decode_attention_args_t a, int ctas)
+template <typename Q, int D, bool WIDE, int NT>
+__global__ void __launch_bounds__(NT * D * kJoinGroups) mf_decode_join_kernel(const __grid_constant__ mf_decode_attention_args_t a, int ctas)
 {
+    constexpr int kRows = 8 * NT;
     GridDependency();
     const int2 *marks = (const int2 *)a.marks;
     const int c = blockIdx.x;
@@ -505,32 +613,71 @@ __global__ void __launch_bounds__(kRows * 16) mf_decode_join_kernel(const __grid
         return;
     }
     const int GT = (a.group + kRows - 1) / kRows, kvh = row.y / GT, g = (row.y % GT) * kRows;
-    const int r = threadIdx.x / (D / 8), d = (threadIdx.x % (D / 8)) * 8;
-    int n = 1;
-    while (c + n < ctas) {
-        const int2 m = marks[2 * (c + n)];
-        if (m.x != row.x || m.y != row.y) {
-            break;
-        }
-        n++;
+    const int group = threadIdx.x / (NT * D), r = threadIdx.x % (NT * D) / (D / 8), d = (threadIdx.x % (D / 8)) * 8;
+    // the CTAs behind that hold a part of the row: all marks at once
+    __shared__ int behind;
+    if (threadIdx.x == 0) {
+        behind = ctas;
     }
+    __syncthreads();
+    for (int i = c + 1 + threadIdx.x; i < ctas; i += blockDim.x) {
+        const int2 m = marks[2 * i];
+        if (m.x != row.x || m.y != row.y) {
+            atomicMin(&behind, i);
+        }
+    }
+    __syncthreads();
+    const int n = behind - c;
     float best = -INFINITY, all = 0, out[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int i = 0; i < n; i++) {
-        const float *ws = Partial<D>((float *)a.workspace, c + i, i == 0 ? 1 : 0);
-        const float2 ms = *(const float2 *)(ws + r * kPartialFloats);
-        const float4 x = *(const float4 *)(ws + kRows * kPartialFloats + r * D + d), y = *(const float4 *)(ws + kRows * kPartialFloats + r * D + d + 4);
-        const float next = fmaxf(best, ms.x), base = next == -INFINITY ? 0.0f : next;
-        const float keep = Exp2(best - base), weight = Exp2(ms.x - base);
-        const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    constexpr int kAhead = 4;  // parts whose loads are in flight together
+    const int from = n * group / kJoinGroups, to = n * (group + 1) / kJoinGroups;  // in order: a group's parts lie before the next one's
+    for (int i = from; i < to; i += kAhead) {
+        float2 ms[kAhead];
+        float4 x[kAhead], y[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            const float *ws = Partial<D, kRows>((float *)a.workspace, c + min(i + u, to - 1), min(i + u, to - 1) == 0 ? 1 : 0);
+            ms[u] = *(const float2 *)(ws + r * kPartialFloats);
+            x[u] = *(const float4 *)(ws + kRows * kPartialFloats + r * D + d);
+            y[u] = *(const float4 *)(ws + kRows * kPartialFloats + r * D + d + 4);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            if (i + u < to) {
+                const float next = fmaxf(best, ms[u].x), base = next == -INFINITY ? 0.0f : next;
+                const float keep = Exp2(best - base), weight = Exp2(ms[u].x - base);
+                const float v[8] = {x[u].x, x[u].y, x[u].z, x[u].w, y[u].x, y[u].y, y[u].z, y[u].w};
+                best = next;
+                all = all * keep + ms[u].y * weight;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    out[j] = out[j] * keep + v[j] * weight;
+                }
+            }
+        }
+    }
+    __shared__ float tops[kJoinGroups][kRows], sums[kJoinGroups][kRows];
+    __shared__ __align__(16) float values[kJoinGroups][kRows * D];
+    if (d == 0) {
+        tops[group][r] = best;
+        sums[group][r] = all;
+    }
+    *(float4 *)&values[group][r * D + d] = make_float4(out[0], out[1], out[2], out[3]);
+    *(float4 *)&values[group][r * D + d + 4] = make_float4(out[4], out[5], out[6], out[7]);
+    __syncthreads();
+    if (group != 0 || g + r >= a.group) {
+        return;
+    }
+#pragma unroll
+    for (int i = 1; i < kJoinGroups; i++) {
+        const float next = fmaxf(best, tops[i][r]), base = next == -INFINITY ? 0.0f : next;
+        const float keep = Exp2(best - base), weight = Exp2(tops[i][r] - base);
         best = next;
-        all = all * keep + ms.y * weight;
+        all = all * keep + sums[i][r] * weight;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            out[j] = out[j] * keep + v[j] * weight;
+            out[j] = out[j] * keep + values[i][r * D + d + j] * weight;
         }
-    }
-    if (g + r >= a.group) {
-        return;
     }
     const int h = kvh * a.group + g + r;
     const float scale = (all != 0 ? 1.0f / all : 0.0f) * (WIDE ? a.vScale[kvh] : 1.0f);
@@ -542,20 +689,34 @@ __global__ void __launch_bounds__(kRows * 16) mf_decode_join_kernel(const __grid
     }
 }
 
-template <typename Q, typename C, int D>
+// Eights of query heads that are worked on together: two where the group has more than eight, which read a key once for both.
+int Eights(int group) { return group > 8 ? 2 : 1; }
+
+int Ctas(int B, int kvHeads, int group, long long capacity)
+{
+    const int sms = mf_k_sm_count(), rows = 8 * Eights(group);
+    const long long tiles = (long long)B * kvHeads * ((group + rows - 1) / rows) * ((capacity + 63) / 64),  // tiles have 64 keys or more
+                    most = (long long)kCtasPerSm * (sms > 0 ? sms : 1);
+    return (int)(tiles < most ? (tiles > 1 ? tiles : 1) : most);
+}
+
+size_t PartialBytes(int ctas, int group, int D) { return (size_t)ctas * 2 * 8 * Eights(group) * (D + kPartialFloats) * sizeof(float); }
+
+template <typename Q, typename C, int D, int NT>
 int Launch(const mf_decode_attention_args_t &a, int ctas, cudaStream_t stream)
 {
-    using X = Cfg<C, D>;
-    if (!mf::AllowSmem<mf_decode_attention_kernel<Q, C, D>>(X::kSmem)) {
+    using X = Cfg<C, D, NT>;
+    constexpr uint32_t kSmem = X::kSmem;
+    if (!mf::AllowSmem<mf_decode_attention_kernel<Q, C, D, NT>>(kSmem)) {
         return MF_K_LAUNCH_FAILED;
     }
-    if (mf::sm100::LaunchDependent(mf_decode_attention_kernel<Q, C, D>, ctas, kThreads, X::kSmem, stream, a) != cudaSuccess) {
+    if (mf::sm100::LaunchDependent(mf_decode_attention_kernel<Q, C, D, NT>, ctas, kThreads, kSmem, stream, a) != cudaSuccess) {
         (void)cudaGetLastError();
         return MF_K_LAUNCH_FAILED;
     }
-    // rows of at most kWholeTiles tiles are never cut
-    if ((long long)a.tableWidth * a.pageSize > kWholeTiles * kTileKeys &&
-        mf::sm100::LaunchDependent(mf_decode_join_kernel<Q, D, sizeof(C) == 1>, ctas, kRows * (D / 8), 0, stream, a, ctas) != cudaSuccess) {
+    // rows of at most kWholeKeys keys are never cut
+    if ((long long)a.tableWidth * a.pageSize > kWholeKeys &&
+        mf::sm100::LaunchDependent(mf_decode_join_kernel<Q, D, sizeof(C) == 1, NT>, ctas, NT * D * kJoinGroups, 0, stream, a, ctas) != cudaSuccess) {
         (void)cudaGetLastError();
         return MF_K_LAUNCH_FAILED;
     }
@@ -565,15 +726,10 @@ int Launch(const mf_decode_attention_args_t &a, int ctas, cudaStream_t stream)
 template <typename Q, typename C>
 int LaunchDim(const mf_decode_attention_args_t &a, int D, int ctas, cudaStream_t stream)
 {
-    return D == 64 ? Launch<Q, C, 64>(a, ctas, stream) : Launch<Q, C, 128>(a, ctas, stream);
-}
-
-int Ctas(int B, int kvHeads, int group, long long capacity)
-{
-    const int sms = mf_k_sm_count();
-    const long long rows = (long long)B * kvHeads * ((group + kRows - 1) / kRows), tiles = rows * ((capacity + kTileKeys - 1) / kTileKeys);
-    const long long most = 2ll * (sms > 0 ? sms : 1);
-    return (int)(tiles < most ? (tiles > 1 ? tiles : 1) : most);
+    if (Eights(a.group) == 1) {
+        return D == 64 ? Launch<Q, C, 64, 1>(a, ctas, stream) : Launch<Q, C, 128, 1>(a, ctas, stream);
+    }
+    return D == 64 ? Launch<Q, C, 64, 2>(a, ctas, stream) : Launch<Q, C, 128, 2>(a, ctas, stream);
 }
 
 }  // namespace
@@ -583,8 +739,8 @@ extern "C" size_t mf_k_decode_attention_workspace(int B, int kvHeads, int group,
     if (B <= 0 || kvHeads <= 0 || group <= 0 || (D != 64 && D != 128) || capacity < 0) {
         return 0;
     }
-    const size_t ctas = (size_t)Ctas(B, kvHeads, group, capacity);
-    return ctas * 2 * (kRows * (D + kPartialFloats) * sizeof(float) + sizeof(int2));
+    const int ctas = Ctas(B, kvHeads, group, capacity);
+    return PartialBytes(ctas, group, D) + (size_t)ctas * 2 * sizeof(int2);
 }
 
 extern "C" int mf_k_decode_attention(const mf_decode_attention_args_t *args, int D, int qType, int cacheType, mf_stream_t stream)
@@ -597,12 +753,20 @@ extern "C" int mf_k_decode_attention(const mf_decode_attention_args_t *args, int
         return MF_K_OK;
     }
     mf_decode_attention_args_t a = *args;
+    // key / pageSize = umulhi(key, pageMagic) >> pageShift for keys below 2^31: the magic number of T. Granlund, P. Montgomery, "Division by
+    // invariant integers using multiplication", 1994, with l = ceil(log2(pageSize)) and one bit less, as the keys have 31. A
+    // page size of 1 would need 33 bits.
+    a.pageShift = 0;
+    while ((1ll << (a.pageShift + 1)) < a.pageSize) {
+        a.pageShift++;
+    }
+    a.pageMagic = a.pageSize == 1 ? 0 : (uint32_t)(((1ull << (32 + a.pageShift)) + a.pageSize - 1) / a.pageSize);
     const long long capacity = (long long)a.tableWidth * a.pageSize;
     const int ctas = Ctas(a.B, a.kvHeads, a.group, capacity);
     if (a.workspace == nullptr) {
         return MF_K_INVALID;
     }
-    a.marks = (unsigned char *)a.workspace + (size_t)ctas * 2 * kRows * (D + kPartialFloats) * sizeof(float);
+    a.marks = (unsigned char *)a.workspace + PartialBytes(ctas, a.group, D);
     if (qType == MF_K_BF16 && cacheType == MF_K_BF16) {
         return LaunchDim<__nv_bfloat16, __nv_bfloat16>(a, D, ctas, (cudaStream_t)stream);
     }

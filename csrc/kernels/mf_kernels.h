@@ -272,6 +272,8 @@ typedef struct {
     long long tableStride;
     int B, kvHeads, group, pageSize, pages, tableWidth, tableRows;
     float scale;
+    unsigned pageMagic;  // set by the launcher
+    int pageShift;       // set by the launcher
 } mf_decode_attention_args_t;
 size_t mf_k_decode_attention_workspace(int B, int kvHeads, int group, int D, long long capacity);
 int mf_k_decode_attention(const mf_decode_attention_args_t *args, int D, int qType, int cacheType, mf_stream_t stream);
