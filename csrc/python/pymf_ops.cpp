@@ -64,6 +64,16 @@ struct MoePlan {
     }
 };
 
+struct DecodePlan {
+    mf_decode_attention_args_t a{};
+    int dim{0}, qType{0}, cacheType{0};
+};
+
+struct PrefillPlan {
+    mf_prefill_attention_args_t a{};
+    int dim{0}, type{0};
+};
+
 }  // namespace
 
 void BindOps(py::module_ &m)
@@ -295,72 +305,88 @@ void BindOps(py::module_ &m)
     ops.attr("FP16") = (int)MF_K_FP16;
     ops.attr("E4M3") = (int)MF_K_E4M3;
     ops.attr("KV_MAX_SEQS") = (int)MF_KV_MAX_SEQS;
-    ops.def("decode_attention_workspace", &mf_k_decode_attention_workspace, py::arg("B"), py::arg("kv_heads"), py::arg("group"), py::arg("D"),
-            py::arg("capacity"));
-    ops.def("decode_attention", [](uint64_t q, uint64_t k, uint64_t v, uint64_t table, uint64_t lengths, uint64_t rows, uint64_t kScale, uint64_t vScale,
-                                   uint64_t out, uint64_t lse, uint64_t status, uint64_t workspace, int64_t qs0, int64_t qs1, int64_t os0, int64_t os1,
-                                   int64_t s0, int64_t s1, int64_t s2, int64_t tableStride, int B, int kvHeads, int group, int pageSize, int pages,
-                                   int tableWidth, int tableRows, float scale, int D, int qType, int cacheType, uint64_t stream) {
-        mf_decode_attention_args_t a{};
-        a.q = (const void *)q;
-        a.k = (const void *)k;
-        a.v = (const void *)v;
-        a.table = (const int *)table;
-        a.lengths = (const int *)lengths;
-        a.rows = (const int *)rows;
-        a.kScale = (const float *)kScale;
-        a.vScale = (const float *)vScale;
-        a.out = (void *)out;
-        a.lse = (float *)lse;
-        a.status = (int *)status;
-        a.workspace = (void *)workspace;
-        a.qStride[0] = qs0;
-        a.qStride[1] = qs1;
-        a.outStride[0] = os0;
-        a.outStride[1] = os1;
-        a.stride[0] = s0;
-        a.stride[1] = s1;
-        a.stride[2] = s2;
-        a.tableStride = tableStride;
-        a.B = B;
-        a.kvHeads = kvHeads;
-        a.group = group;
-        a.pageSize = pageSize;
-        a.pages = pages;
-        a.tableWidth = tableWidth;
-        a.tableRows = tableRows;
-        a.scale = scale;
-        return mf_k_decode_attention(&a, D, qType, cacheType, (mf_stream_t)stream);
-    });
-    ops.def("prefill_attention", [](uint64_t q, uint64_t k, uint64_t v, uint64_t cuQ, uint64_t cuK, uint64_t out, uint64_t lse, uint64_t status, int64_t qs0, int64_t qs1,
-                                    int64_t ks0, int64_t ks1, int64_t vs0, int64_t vs1, int64_t os0, int64_t os1, int B, int kvHeads, int group, int tokensQ,
-                                    int tokensK, int causal, float scale, int D, int type, uint64_t stream) {
-        mf_prefill_attention_args_t a{};
-        a.q = (const void *)q;
-        a.k = (const void *)k;
-        a.v = (const void *)v;
-        a.cuQ = (const int *)cuQ;
-        a.cuK = (const int *)cuK;
-        a.out = (void *)out;
-        a.lse = (float *)lse;
-        a.status = (int *)status;
-        a.qStride[0] = qs0;
-        a.qStride[1] = qs1;
-        a.kStride[0] = ks0;
-        a.kStride[1] = ks1;
-        a.vStride[0] = vs0;
-        a.vStride[1] = vs1;
-        a.outStride[0] = os0;
-        a.outStride[1] = os1;
-        a.B = B;
-        a.kvHeads = kvHeads;
-        a.group = group;
-        a.tokensQ = tokensQ;
-        a.tokensK = tokensK;
-        a.causal = causal;
-        a.scale = scale;
-        return mf_k_prefill_attention(&a, D, type, (mf_stream_t)stream);
-    });
+    // Shapes and strides of a call; its addresses come with run().
+    py::class_<DecodePlan>(ops, "DecodePlan")
+        .def(py::init([](int64_t qs0, int64_t qs1, int64_t os0, int64_t os1, int64_t s0, int64_t s1, int64_t s2, int64_t tableStride, int B, int kvHeads,
+                         int group, int pageSize, int pages, int tableWidth, int tableRows, int D, int qType, int cacheType) {
+            DecodePlan p;
+            p.a.qStride[0] = qs0;
+            p.a.qStride[1] = qs1;
+            p.a.outStride[0] = os0;
+            p.a.outStride[1] = os1;
+            p.a.stride[0] = s0;
+            p.a.stride[1] = s1;
+            p.a.stride[2] = s2;
+            p.a.tableStride = tableStride;
+            p.a.B = B;
+            p.a.kvHeads = kvHeads;
+            p.a.group = group;
+            p.a.pageSize = pageSize;
+            p.a.pages = pages;
+            p.a.tableWidth = tableWidth;
+            p.a.tableRows = tableRows;
+            p.dim = D;
+            p.qType = qType;
+            p.cacheType = cacheType;
+            return p;
+        }))
+        .def("workspace", [](const DecodePlan &p) {
+            return mf_k_decode_attention_workspace(p.a.B, p.a.kvHeads, p.a.group, p.dim, (long long)p.a.tableWidth * p.a.pageSize);
+        })
+        .def("run", [](const DecodePlan &p, uint64_t q, uint64_t k, uint64_t v, uint64_t out, uint64_t table, uint64_t lengths, uint64_t rows, uint64_t kScale,
+                       uint64_t vScale, uint64_t lse, uint64_t status, uint64_t workspace, float scale, uint64_t stream) {
+            mf_decode_attention_args_t a = p.a;
+            a.q = (const void *)q;
+            a.k = (const void *)k;
+            a.v = (const void *)v;
+            a.out = (void *)out;
+            a.table = (const int *)table;
+            a.lengths = (const int *)lengths;
+            a.rows = (const int *)rows;
+            a.kScale = (const float *)kScale;
+            a.vScale = (const float *)vScale;
+            a.lse = (float *)lse;
+            a.status = (int *)status;
+            a.workspace = (void *)workspace;
+            a.scale = scale;
+            return mf_k_decode_attention(&a, p.dim, p.qType, p.cacheType, (mf_stream_t)stream);
+        });
+    py::class_<PrefillPlan>(ops, "PrefillPlan")
+        .def(py::init([](int64_t qs0, int64_t qs1, int64_t ks0, int64_t ks1, int64_t vs0, int64_t vs1, int64_t os0, int64_t os1, int B, int kvHeads, int group,
+                         int tokensQ, int tokensK, int D, int type) {
+            PrefillPlan p;
+            p.a.qStride[0] = qs0;
+            p.a.qStride[1] = qs1;
+            p.a.kStride[0] = ks0;
+            p.a.kStride[1] = ks1;
+            p.a.vStride[0] = vs0;
+            p.a.vStride[1] = vs1;
+            p.a.outStride[0] = os0;
+            p.a.outStride[1] = os1;
+            p.a.B = B;
+            p.a.kvHeads = kvHeads;
+            p.a.group = group;
+            p.a.tokensQ = tokensQ;
+            p.a.tokensK = tokensK;
+            p.dim = D;
+            p.type = type;
+            return p;
+        }))
+        .def("run", [](const PrefillPlan &p, uint64_t q, uint64_t k, uint64_t v, uint64_t out, uint64_t cuQ, uint64_t cuK, uint64_t lse, uint64_t status, bool causal,
+                       float scale, uint64_t stream) {
+            mf_prefill_attention_args_t a = p.a;
+            a.q = (const void *)q;
+            a.k = (const void *)k;
+            a.v = (const void *)v;
+            a.out = (void *)out;
+            a.cuQ = (const int *)cuQ;
+            a.cuK = (const int *)cuK;
+            a.lse = (float *)lse;
+            a.status = (int *)status;
+            a.causal = causal ? 1 : 0;
+            a.scale = scale;
+            return mf_k_prefill_attention(&a, p.dim, p.type, (mf_stream_t)stream);
+        });
     // The tensors of a paged key-value cache, and the launches on it.
     py::class_<mf_kv_cache_t>(ops, "KvCache")
         .def(py::init([](uint64_t data, uint64_t table, uint64_t lengths, uint64_t refs, uint64_t status, int layers, int pages, int pageSize, int kvHeads,
