@@ -104,6 +104,13 @@ __device__ __forceinline__ float2 Unpack2<__half>(uint32_t v)
     return __half22float2(*reinterpret_cast<const __half2 *>(&v));
 }
 
+// Where the reference of a row's weights lies, in powers of two: kLift below its maximum when it is set, and set anew when a weight would pass 2^kSlack.
+// fp16 weights are lifted so that those of a thousandth and less of the largest are not subnormal.
+template <typename T>
+struct Weights {
+    static constexpr float kLift = Bf16<T>::value ? 0.0f : 6.0f, kSlack = Bf16<T>::value ? 8.0f : 14.0f;
+};
+
 // Two e4m3 values (low 16 bits) as a pair of fp16, which holds all of them exactly.
 __device__ __forceinline__ uint32_t E4m3ToHalf2(uint32_t v)
 {

@@ -16,8 +16,8 @@
 // of cp.async stages (rows past the end of the sequence are filled with zeros: stale pages may hold anything, NaN included) and keeps its
 // own maximum and sum; they meet at the end of a row. Products are m16n8k16 with the keys (then the columns of v) as the 16 rows and eight
 // query heads as the columns, so a group of up to eight heads costs one product per 16 x 16 values of the cache and all statistics of a
-// head lie in the lanes that hold its results. The reference of the exponentials follows the maximum only where that has grown by more
-// than 2^8 (p stays below 256): most tiles need one vote for it, no shuffles and no scaling of the output.
+// head lie in the lanes that hold its results. The reference of the exponentials follows the maximum only where a weight
+// would pass 2^8 (fp16: 2^14): most tiles need one vote for it, no shuffles and no scaling of the output.
 //
 // 8-bit caches are widened to fp16, which holds every e4m3 value; the query is scaled by a power of two per head so that it fits fp16
 // without loss. p is rounded to the cache's type (fp16 for 8-bit caches) for the second product, as the tensor cores want equal
@@ -41,7 +41,6 @@ constexpr int kRowCost = 3;        // tiles that beginning and ending a row take
 constexpr int kPartialFloats = 2;  // maximum and sum before a row's values
 constexpr int kLeastPiece = 2;
 constexpr int kJoinGroups = 4;     // of threads that share the parts of a row in the second kernel
-constexpr float kSlack = 8.0f;     // powers of two by which the reference may lag behind the maximum
 
 template <typename C, int D, int NT>
 struct Cfg {
@@ -417,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) mf_decode_attention_kern
                     for (int e = 0; e < 4; e++) {
                         const bool seen = key0 + block * 16 + quad + (e >> 1) * 8 < cur.length;
                         x[block][t][e] = seen ? (y[0][t][e] + y[1][t][e]) * factor[t][e & 1] : -INFINITY;
-                        grown |= x[block][t][e] - top[t][e & 1] > kSlack;
+                        grown |= x[block][t][e] - top[t][e & 1] > Weights<T>::kSlack;
                     }
                 }
             }
@@ -426,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) mf_decode_attention_kern
                 for (int t = 0; t < NT; t++) {
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        float best = top[t][e];
+                        float best = top[t][e] + Weights<T>::kLift;
 #pragma unroll
                         for (int block = 0; block < kBlocks; block++) {
                             best = fmaxf(best, fmaxf(x[block][t][e], x[block][t][e + 2]));
@@ -434,6 +433,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) mf_decode_attention_kern
                         best = fmaxf(best, __shfl_xor_sync(~0u, best, 4));
                         best = fmaxf(best, __shfl_xor_sync(~0u, best, 8));
                         best = fmaxf(best, __shfl_xor_sync(~0u, best, 16));
+                        best -= Weights<T>::kLift;
                         const float shrink = Exp2(top[t][e] - (best == -INFINITY ? 0.0f : best));
                         top[t][e] = best;
                         sum[t][e] *= shrink;

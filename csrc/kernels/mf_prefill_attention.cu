@@ -13,12 +13,11 @@
 //                    the P that the second overwrites, and the tensor core takes them in order.
 //   warp 9           TMA: both Q tiles, then keys and values in turn through a ring of stages.
 //
-// The reference m only follows the maximum where that has grown by more than 2^8 since (p stays below 256, sums far below
-// overflow); then the row's O is scaled in TMEM. That is rare, so no warps are kept for it. The S barrier of a key tile stands for the
+// The reference m only follows the maximum where a weight would pass 2^8 (fp16: 2^14); then the row's O is scaled in TMEM. That is rare, so no warps are kept for it. The S barrier of a key tile stands for the
 // completion of all MMAs before it, so O is at rest when its S arrives.
 //
-// p is rounded to the operands' type for the second product (the tensor core wants one type for both); the sum is taken before that, all
-// sums and O are fp32. A masked key counts 0 * v in a tile product, which is not 0 where v is infinite or NaN: a row whose result is not finite
+// p is rounded to the operands' type for the second product (the tensor core wants one type for both); the sum is taken before
+// that, all sums and O are fp32. A masked key counts 0 * v in a tile product, which is not 0 where v is infinite or NaN: a row whose result is not finite
 // is computed again key by key. All waits are bounded; one that runs out sets the status, and the CTA drains and leaves.
 #include <cuda.h>
 
@@ -35,7 +34,6 @@ using namespace mf::sm100;
 constexpr int kTile = 128;  // rows of a tile, keys of a tile
 constexpr int kThreads = 384;
 constexpr uint32_t kHalf = kTile * 128;  // bytes of 64 columns of a tile
-constexpr float kSlack = 8.0f;           // powers of two by which the reference may lag behind the maximum
 constexpr int kEarly = 96;               // keys whose P is handed over while the others are still computed
 // Registers of a softmax thread, which holds a row of S, and of the others: 256 * 200 + 128 * 96 of the 384 * 168 of the launch.
 constexpr int kSoftmaxRegs = 200, kOtherRegs = 96;
@@ -432,7 +430,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
         const int i = warp >> 2;  // the tile
         const int row = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, sAt = tmem + lanes + i * kTile, oAt = tmem + lanes + kO + i * D;
-        const float factor = a.scale * kLog2e;
+        const float factor = a.scale * kLog2e, lift = Weights<T>::kLift / factor;
         Worker<D> worker;
         Work w;
         uint32_t sPh = 0, oPh = 0;
@@ -483,10 +481,10 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                     m[e] = fmaxf(m[e], x[kTile - 4 + e]);
                 }
                 const float best = Max3(fmaxf(m[0], m[1]), m[2], m[3]);
-                const bool grown = (best - top) * factor > kSlack;
+                const bool grown = (best - top) * factor > Weights<T>::kSlack;
                 if (__any_sync(~0u, grown)) {
-                    const float shrink = grown ? Exp2((top - best) * factor) : 1.0f;
-                    top = grown ? best : top;
+                    const float shrink = grown ? Exp2((top - best + lift) * factor) : 1.0f;
+                    top = grown ? best - lift : top;
                     sum *= shrink;
                     if (j > 0) {
 #pragma unroll
