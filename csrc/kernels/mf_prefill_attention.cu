@@ -21,6 +21,8 @@
 // is computed again key by key. All waits are bounded; one that runs out sets the status, and the CTA drains and leaves.
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "mf_attention.cuh"
 #include "mf_kernels.h"
 #include "mf_launch.cuh"
@@ -52,6 +54,8 @@ struct Shared {
     unsigned char q[2][kTileBytes];
     unsigned char kv[kStages][kTileBytes];
     uint64_t qFull, qEmpty, kvFull[kStages], kvEmpty[kStages], sFull[2], pFull[2], pRest[2], oFull[2], workFull[2], workEmpty[2];
+    uint4 claim;  // the answer to Claim()
+    uint64_t claimed;
     Work work[2];
     uint32_t tmem;
     int abortFlag;
@@ -64,7 +68,6 @@ struct Params {
     int wide;      // output rows begin at multiples of 32 bytes: whole sectors are stored
     int headTiles; // kvHeads * group / pack
     int tiles;     // numbers of row tiles, empty ones among them
-    int units;     // tiles * headTiles
 };
 
 __device__ __forceinline__ float Max3(float a, float b, float c)
@@ -95,6 +98,12 @@ __device__ __forceinline__ uint64_t Add2(uint64_t a, uint64_t b)
 {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t Mul2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 __device__ __forceinline__ float AtLeast(float x, float least)
@@ -148,6 +157,121 @@ __device__ __forceinline__ void FewerRegisters()
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
+// Asks for a CTA of this grid that has not been launched yet, in the place of which the caller will work; 16 bytes of answer come to `answer` and are counted on `bar`.
+__device__ __forceinline__ void ClaimCta(uint4 *answer, uint64_t *bar)
+{
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(SmemAddr(answer)), "r"(SmemAddr(bar))
+                 : "memory");
+}
+// Its blockIdx.x, or -1 if all have been launched.
+__device__ __forceinline__ int ClaimedCta(const uint4 *answer)
+{
+    int x;
+    asm volatile(
+        "{\n.reg .b128 h;\n.reg .pred p;\n"
+        "ld.shared.b128 h, [%1];\n"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+        "mov.b32 %0, -1;\n"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, h;\n}\n"
+        : "=r"(x)
+        : "r"(SmemAddr(answer))
+        : "memory");
+    return x;
+}
+
+// Sequence b's query rows and keys, as far as there are tokens.
+__device__ __forceinline__ void Extent(const mf_prefill_attention_args_t &a, int b, Work &w)
+{
+    w.q0 = a.cuQ[b];
+    w.rows = w.q0 < 0 ? 0 : min(a.cuQ[b + 1], a.tokensQ) - w.q0;
+    w.k0 = a.cuK[b];
+    w.keys = w.k0 < 0 ? 0 : min(a.cuK[b + 1], a.tokensK) - w.k0;
+}
+
+// Row tiles of sequence b have numbers from cuQ[b] / tokens + b on: enough for its rows wherever they begin, some numbers stay empty. Taken from
+// the end, as the last tiles of a causal prompt are the longest. Whole warp; false: an empty number.
+__device__ __forceinline__ bool Numbered(const Params &p, int number, Work &w)
+{
+    const mf_prefill_attention_args_t &a = p.a;
+    const int lane = threadIdx.x & 31, tile = p.tiles - 1 - number;
+    int lo = 0, hi = a.B;  // the last sequence whose first number is not behind `tile`: 32 places at a time
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const unsigned low = __ballot_sync(~0u, at < hi && a.cuQ[at] / p.tokens + at <= tile) | 1u;
+        const int last = 31 - __clz(low);
+        hi = min(hi, lo + (last + 1) * step);
+        lo += last * step;
+    }
+    Extent(a, lo, w);
+    w.t0 = (tile - (w.q0 / p.tokens + lo)) * p.tokens;
+    return w.t0 >= 0 && w.t0 < w.rows;
+}
+
+// The same for a few sequences, with the row tiles in order of the key tiles that they take, the most first: what is left at the end is small. How many
+// row tiles take m key tiles or more follows from a sequence's lengths; the m of a number is found by bisection. A lane has two sequences.
+constexpr int kRanked = 64;
+__device__ __forceinline__ bool Ranked(const Params &p, int number, Work &w)
+{
+    const mf_prefill_attention_args_t &a = p.a;
+    const int lane = threadIdx.x & 31;
+    Work seq[2];
+    int tiles[2], most = 0;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int b = lane * 2 + i;
+        seq[i].rows = seq[i].keys = 0;
+        if (b < a.B) {
+            Extent(a, b, seq[i]);
+        }
+        tiles[i] = seq[i].rows > 0 ? (seq[i].rows + p.tokens - 1) / p.tokens : 0;
+        most = max(most, seq[i].keys > 0 ? (seq[i].keys + kTile - 1) / kTile : 0);
+    }
+    // the first row tile of a sequence that takes m key tiles or more (its number of row tiles, if none does)
+    auto first = [&](int i, int m) {
+        const int need = (m - 1) * kTile + 1, past = seq[i].keys - seq[i].rows;
+        if (m <= 0) {
+            return 0;
+        }
+        if (seq[i].keys < need) {
+            return tiles[i];
+        }
+        return a.causal ? max(0, min(tiles[i] - 1, (need - past + p.tokens - 1) / p.tokens - 1)) : 0;
+    };
+    auto count = [&](int m) { return __reduce_add_sync(~0u, max(0, tiles[0] - first(0, m)) + max(0, tiles[1] - first(1, m))); };
+    int lo = 0, hi = __reduce_max_sync(~0u, most) + 1;  // count(lo) > number >= count(hi)
+    if (number >= count(0)) {
+        return false;
+    }
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (count(mid) > number) {
+            lo = mid;
+        } else {
+            hi = mid;
+        }
+    }
+    int at = number - count(lo + 1);  // among those that take `lo`
+    const int from[2] = {first(0, lo), first(1, lo)};
+    const int mine[2] = {max(0, first(0, lo + 1) - from[0]), max(0, first(1, lo + 1) - from[1])};
+    int before = mine[0] + mine[1];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(~0u, before, d);
+        before += lane >= d ? y : 0;
+    }
+    before -= mine[0] + mine[1];
+    const int which = at < before + mine[0] ? 0 : 1;
+    const unsigned owner = __ballot_sync(~0u, at >= before && at < before + mine[0] + mine[1]);
+    const int l = __ffs(owner) - 1;
+    at -= before + (which ? mine[0] : 0);
+    w.q0 = __shfl_sync(~0u, which ? seq[1].q0 : seq[0].q0, l);
+    w.rows = __shfl_sync(~0u, which ? seq[1].rows : seq[0].rows, l);
+    w.k0 = __shfl_sync(~0u, which ? seq[1].k0 : seq[0].k0, l);
+    w.keys = __shfl_sync(~0u, which ? seq[1].keys : seq[0].keys, l);
+    w.t0 = __shfl_sync(~0u, ((which ? from[1] : from[0]) + at) * p.tokens, l);
+    return owner != 0 && w.t0 < w.rows;
+}
+
 // A warp's view of the work list: the next two row tiles, or false at its end.
 template <int D>
 struct Worker {
@@ -194,6 +318,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
             MbarInit(&s.workFull[i], 1);
             MbarInit(&s.workEmpty[i], 11);
         }
+        MbarInit(&s.claimed, 1);
         s.abortFlag = 0;
         MbarInitFence();
         TmaPrefetchDesc(&mapQ);
@@ -215,51 +340,42 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
         FewerRegisters<kOtherRegs>();
         if (warp == 10) {
             // ------------------------------------------------------------------ scheduler
-            // Row tiles of sequence b have numbers from cuQ[b] / tokens + b on: enough for its rows wherever they begin, some numbers stay empty. The
-            // last tiles of a causal prompt are the longest, so numbers are dealt out from the end, there and back over the CTAs.
+            // Each unit of work is a CTA of the grid; a CTA that runs takes the next one that has not been launched yet when it begins with the one before.
             int k = 0;
-            for (int round = 0;; round++) {
-                const long long unit = (long long)round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-                const bool end = (long long)round * gridDim.x >= p.units;
+            long long unit = blockIdx.x;
+            for (uint32_t claims = 0;; claims++) {
+                const bool end = unit < 0;
+                const int ht = (int)(unit % p.headTiles), number = (int)(unit / p.headTiles);
                 Work w = {0, 0, 0, 0, 0, -1, 0, 0};
-                if (!end) {
-                    if (unit >= p.units) {
-                        continue;
-                    }
-                    const int tile = p.tiles - 1 - (int)(unit / p.headTiles), ht = (int)(unit % p.headTiles);
-                    int lo = 0, hi = a.B;  // the last sequence whose first number is not behind `tile`: 32 places at a time
-                    while (hi - lo > 1) {
-                        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-                        const unsigned low = __ballot_sync(~0u, at < hi && a.cuQ[at] / p.tokens + at <= tile) | 1u;
-                        const int last = 31 - __clz(low);
-                        hi = min(hi, lo + (last + 1) * step);
-                        lo += last * step;
-                    }
-                    w.q0 = a.cuQ[lo];
-                    w.rows = min(a.cuQ[lo + 1], a.tokensQ) - w.q0;
-                    w.t0 = (tile - (w.q0 / p.tokens + lo)) * p.tokens;
-                    if (w.q0 < 0 || w.t0 < 0 || w.t0 >= w.rows) {
-                        continue;
-                    }
-                    w.k0 = a.cuK[lo];
-                    w.keys = w.k0 < 0 ? 0 : min(a.cuK[lo + 1], a.tokensK) - w.k0;
+                const bool there = !end && (a.B <= kRanked ? Ranked(p, number, w) : Numbered(p, number, w));
+                if (there) {
                     const int see = a.causal ? min(w.keys, min(w.rows, w.t0 + p.tokens) + w.keys - w.rows) : w.keys;
                     w.n = see > 0 ? (see + kTile - 1) / kTile : 0;
                     const int perKv = a.group / p.pack;
                     w.kvh = ht / perKv;
                     w.h0 = w.kvh * a.group + (ht % perKv) * p.pack;
                 }
-                if (!MbarWaitWarp(&s.workEmpty[k & 1], ((k >> 1) & 1) ^ 1, abortFlag)) {
-                    break;
+                if (there || end) {
+                    if (lane == 0) {
+                        s.work[k & 1] = w;
+                        MbarArrive(&s.workFull[k & 1]);
+                    }
+                    if (end || !MbarWaitWarp(&s.workEmpty[k & 1], (k >> 1) & 1, abortFlag)) {  // so the other place is free, too
+                        break;
+                    }
+                    k++;
                 }
                 if (lane == 0) {
-                    s.work[k & 1] = w;
-                    MbarArrive(&s.workFull[k & 1]);
+                    MbarExpectTx(&s.claimed, 16);
+                    ClaimCta(&s.claim, &s.claimed);
                 }
-                k++;
-                if (end) {
+                int own = 0;  // the answer is waited for even if the CTA gives up: it is written to its shared memory
+                if (!MbarWaitWarp(&s.claimed, claims & 1, &own)) {
+                    *abortFlag = 1;
                     break;
                 }
+                unit = ClaimedCta(&s.claim);
+                FenceProxyAsyncShared();
             }
         } else if (warp == 9) {
             // ------------------------------------------------------------------ TMA producer
@@ -431,81 +547,64 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
         const int row = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, sAt = tmem + lanes + i * kTile, oAt = tmem + lanes + kO + i * D;
         const float factor = a.scale * kLog2e, lift = Weights<T>::kLift / factor;
-        Worker<D> worker;
-        Work w;
-        uint32_t sPh = 0, oPh = 0;
-        bool ok = true;
-        while (ok && worker.Next(s, abortFlag, w)) {
-            if (i == 1 && w.t0 + half >= w.rows) {
-                continue;
+        float top = -INFINITY, sum = 0;
+        // One key tile. CUT: the row sees its first `left` columns only, no row of the warp sees any from `cols` on.
+        auto tile = [&](auto cut, bool first, int left, int cols) {
+            constexpr bool kCut = decltype(cut)::value;
+            float x[kTile];
+#pragma unroll
+            for (int c = 0; c < kTile; c += 32) {
+                TmemLd32Issue(sAt + c, x + c);
             }
-            // rows that the packing leaves over hold anything, and nobody looks at them
-            const int token = row < p.pack * half ? w.t0 + i * half + row / p.pack : 0x7fffffff, past = w.keys - w.rows;
-            const bool valid = token < w.rows;
-            const int limit = a.causal && valid ? min(w.keys, token + past + 1) : w.keys;  // keys that the row sees
-            const int sure = __reduce_min_sync(~0u, limit);
-            float top = -INFINITY, sum = 0;
-            for (int j = 0; j < w.n; j++) {
-                if (!MbarWaitWarp(&s.sFull[i], sPh, abortFlag)) {
-                    ok = false;
-                    break;
-                }
-                sPh ^= 1;
-                TcFenceAfter();
-                float x[kTile];
 #pragma unroll
-                for (int c = 0; c < kTile; c += 32) {
-                    TmemLd32Issue(sAt + c, x + c);
-                }
+            for (int c = 0; c < kTile; c += 32) {
+                TmemLdWait32(x + c);
+            }
+            if (kCut) {
 #pragma unroll
-                for (int c = 0; c < kTile; c += 32) {
-                    TmemLdWait32(x + c);
+                for (int c = 0; c < kTile; c++) {
+                    x[c] = c < left ? x[c] : -INFINITY;
                 }
-                if ((j + 1) * kTile > sure) {
-                    const int left = limit - j * kTile;
+            }
+            float m[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                    for (int c = 0; c < kTile; c++) {
-                        x[c] = c < left ? x[c] : -INFINITY;
-                    }
-                }
-                float m[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                for (int c = 4; c < kTile - 4; c += 8) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        m[e] = Max3(m[e], x[c + e], x[c + 4 + e]);
-                    }
-                }
+            for (int c = 4; c < kTile - 4; c += 8) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    m[e] = fmaxf(m[e], x[kTile - 4 + e]);
+                    m[e] = Max3(m[e], x[c + e], x[c + 4 + e]);
                 }
-                const float best = Max3(fmaxf(m[0], m[1]), m[2], m[3]);
-                const bool grown = (best - top) * factor > Weights<T>::kSlack;
-                if (__any_sync(~0u, grown)) {
-                    const float shrink = grown ? Exp2((top - best + lift) * factor) : 1.0f;
-                    top = grown ? best - lift : top;
-                    sum *= shrink;
-                    if (j > 0) {
+            }
 #pragma unroll
-                        for (int c = 0; c < D; c += 16) {
-                            float o[16];
-                            TmemLd16Issue(oAt + c, o);
-                            TmemLdWait16(o);
+            for (int e = 0; e < 4; e++) {
+                m[e] = fmaxf(m[e], x[kTile - 4 + e]);
+            }
+            const float best = Max3(fmaxf(m[0], m[1]), m[2], m[3]);
+            const bool grown = (best - top) * factor > Weights<T>::kSlack;
+            if (__any_sync(~0u, grown)) {
+                const float shrink = grown ? Exp2((top - best + lift) * factor) : 1.0f;
+                top = grown ? best - lift : top;
+                sum *= shrink;
+                if (!first) {
 #pragma unroll
-                            for (int e = 0; e < 16; e++) {
-                                o[e] *= shrink;
-                            }
-                            TmemSt16(oAt + c, (const uint32_t *)o);
+                    for (int c = 0; c < D; c += 16) {
+                        float o[16];
+                        TmemLd16Issue(oAt + c, o);
+                        TmemLdWait16(o);
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            o[e] *= shrink;
                         }
+                        TmemSt16(oAt + c, (const uint32_t *)o);
                     }
                 }
-                const float from = top == -INFINITY ? 0.0f : -top * factor;
-                const uint64_t factor2 = Both(factor, factor), from2 = Both(from, from);
-                uint64_t part[2] = {0, 0};
+            }
+            const float from = top == -INFINITY ? 0.0f : -top * factor;
+            const uint64_t factor2 = Both(factor, factor), from2 = Both(from, from);
+            uint64_t part[2] = {0, 0};
 #pragma unroll
-                for (int c = 0; c < kTile; c += 32) {
-                    uint32_t w16[16];
+            for (int c = 0; c < kTile; c += 32) {
+                uint32_t w16[16];
+                if (!kCut || c < cols) {
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
                         const uint64_t y = Fma2(Both(x[c + 2 * e], x[c + 2 * e + 1]), factor2, from2);
@@ -519,35 +618,63 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                         part[e & 1] = Add2(part[e & 1], Both(u.x, u.y));
                         w16[e] = Pack2<T>(u.x, u.y);
                     }
-                    TmemSt16(sAt + c / 2, w16);
-                    if (c + 32 == kEarly || c + 32 == kTile) {
-                        TmemStWait();
-                        TcFenceBefore();
-                        __syncwarp();
-                        if (lane == 0) {
-                            MbarArrive(c + 32 == kEarly ? &s.pFull[i] : &s.pRest[i]);
-                        }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        w16[e] = 0;
                     }
                 }
-                const float2 both = Apart(Add2(part[0], part[1]));
-                sum += both.x + both.y;
+                TmemSt16(sAt + c / 2, w16);
+                if (c + 32 == kEarly || c + 32 == kTile) {
+                    TmemStWait();
+                    TcFenceBefore();
+                    __syncwarp();
+                    if (lane == 0) {
+                        MbarArrive(c + 32 == kEarly ? &s.pFull[i] : &s.pRest[i]);
+                    }
+                }
             }
-            if (!ok) {
-                break;
+            const float2 both = Apart(Add2(part[0], part[1]));
+            sum += both.x + both.y;
+        };
+        Worker<D> worker;
+        Work w;
+        uint32_t sPh = 0, oPh = 0;
+        bool ok = true;
+        while (ok && worker.Next(s, abortFlag, w)) {
+            if (i == 1 && w.t0 + half >= w.rows) {
+                continue;
             }
-            if (w.n > 0) {
-                if (!MbarWaitWarp(&s.oFull[i], oPh, abortFlag)) {
+            // rows that the packing leaves over hold anything, and nobody looks at them
+            const int token = row < p.pack * half ? w.t0 + i * half + row / p.pack : 0x7fffffff, past = w.keys - w.rows, head = w.h0 + row % p.pack;
+            const bool valid = token < w.rows;
+            const int limit = a.causal && valid ? min(w.keys, token + past + 1) : w.keys;  // keys that the row sees
+            const int sure = __reduce_min_sync(~0u, limit), most = __reduce_max_sync(~0u, valid ? limit : 0);
+            top = -INFINITY;
+            sum = 0;
+            for (int j = 0; j < w.n; j++) {
+                if (!MbarWaitWarp(&s.sFull[i], sPh, abortFlag)) {
+                    ok = false;
                     break;
                 }
-                oPh ^= 1;
+                sPh ^= 1;
                 TcFenceAfter();
+                if ((j + 1) * kTile <= sure) {
+                    tile(std::false_type{}, j == 0, kTile, kTile);
+                } else {
+                    tile(std::true_type{}, j == 0, limit - j * kTile, most - j * kTile);
+                }
             }
-            // A row that saw no key has weights of 2^-126 from Exp2Poly: it is known by its reference.
+            if (!ok || (w.n > 0 && !MbarWaitWarp(&s.oFull[i], oPh, abortFlag))) {
+                break;
+            }
+            oPh ^= w.n > 0 ? 1 : 0;
+            TcFenceAfter();
+            // ---- O / sum. A row that saw no key has weights of 2^-126 from Exp2Poly: it is known by its reference.
             const float scale = top != -INFINITY || sum != sum ? 1.0f / sum : 0.0f;
-            const int head = w.h0 + row % p.pack;
-            const size_t at = (size_t)w.q0 + token;
-            T *out = (T *)a.out + at * a.outStride[0] + (size_t)head * a.outStride[1];
-            bool odd = false;
+            const uint64_t scale2 = Both(scale, scale);
+            T *out = (T *)a.out + ((size_t)w.q0 + token) * a.outStride[0] + (size_t)head * a.outStride[1];
+            uint64_t odd = 0;  // stays 0 as long as what is added is 0 times something finite
 #pragma unroll
             for (int c = 0; c < D; c += 32) {
                 float o[32];
@@ -560,30 +687,30 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                     TmemLdWait32(o);
                 }
 #pragma unroll
-                for (int e = 0; e < 32; e++) {
-                    odd |= !(fabsf(o[e]) <= 3.4e38f);
-                }
-                if (valid) {
+                for (int h = 0; h < 32; h += 16) {
+                    uint32_t pk[8];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 16) {
-                        uint32_t pk[8];
-#pragma unroll
-                        for (int f = 0; f < 8; f++) {
-                            pk[f] = Pack2<T>(o[e + 2 * f] * scale, o[e + 2 * f + 1] * scale);
-                        }
+                    for (int e = 0; e < 8; e++) {
+                        const uint64_t y = Both(o[h + 2 * e], o[h + 2 * e + 1]);
+                        odd = Fma2(y, 0, odd);
+                        const float2 z = Apart(Mul2(y, scale2));
+                        pk[e] = Pack2<T>(z.x, z.y);
+                    }
+                    if (valid) {
                         if (p.wide) {
-                            StGlobal32B(out + c + e, pk);
+                            StGlobal32B(out + c + h, pk);
                         } else {
-                            *(uint4 *)(out + c + e) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-                            *(uint4 *)(out + c + e + 8) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+                            *(uint4 *)(out + c + h) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                            *(uint4 *)(out + c + h + 8) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
                         }
                     }
                 }
             }
             if (a.lse != nullptr && valid) {
-                a.lse[at * a.kvHeads * a.group + head] = top == -INFINITY ? -INFINITY : top * factor * kLn2 + logf(sum);
+                a.lse[((size_t)w.q0 + token) * a.kvHeads * a.group + head] = top == -INFINITY ? -INFINITY : top * factor * kLn2 + logf(sum);
             }
-            unsigned again = __ballot_sync(~0u, odd && valid);
+            const float2 any = Apart(odd);
+            unsigned again = __ballot_sync(~0u, !(any.x + any.y == 0.0f) && valid);
             while (again != 0) {
                 const int r = (warp & 3) * 32 + __ffs(again) - 1, t = w.t0 + i * half + r / p.pack, h = w.h0 + r % p.pack;
                 again &= again - 1;
@@ -652,12 +779,10 @@ int Launch(const mf_prefill_attention_args_t &a, cudaStream_t stream)
     p.headTiles = a.kvHeads * a.group / p.pack;
     p.tiles = a.tokensQ / p.tokens + a.B;
     const long long units = (long long)p.tiles * p.headTiles;
-    const int sms = mf_k_sm_count();
-    if (units > 0x7fffffffll || sms <= 0) {
-        return sms <= 0 ? MF_K_LAUNCH_FAILED : MF_K_TOO_LARGE;
+    if (units > 0x7fffffffll) {
+        return MF_K_TOO_LARGE;
     }
-    p.units = (int)units;
-    const unsigned ctas = units < sms ? (unsigned)units : (unsigned)sms;
+    const unsigned ctas = (unsigned)units;
     CUtensorMap q, k, v;
     constexpr bool kBf16 = Bf16<T>::value;
     // without keys their maps are never used, but have to describe something
