@@ -113,8 +113,8 @@ __device__ __forceinline__ float AtLeast(float x, float least)
     return r;
 }
 
-// 2^x for x <= 16 on the FMA pipe, for a share of the weights: the special function unit gives 16 results a cycle and SM, as long a time for a
-// tile as its MMAs take at D = 128. x = n + f with n the nearest whole number (W. J. Cody, W. Waite, "Software Manual for the Elementary
+// 2^x for x <= 16 on the FMA pipe, for a share of the weights: the special function unit gives 16 results a cycle and SM, which is as long for a tile
+// as its MMAs take at D = 128. x = n + f with n the nearest whole number (W. J. Cody, W. Waite, "Software Manual for the Elementary
 // Functions", 1980), 2^f by the polynomial of least relative error on [-1/2, 1/2] (Remez exchange; 7.5e-5 of degree 3, 2.7e-6 of degree 4,
 // below the rounding of p to bf16 and fp16), n added to its exponent. Below -126 the result stays near 2^-126 (the exponent field must not fall below 0); NaN comes out as an
 // infinite or huge p, which has the row computed again.
@@ -140,11 +140,9 @@ __device__ __forceinline__ float2 Exp2Poly(uint64_t x2)
     return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(r.x) << 23)), __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23)));
 }
 
-// Of four pairs of weights, how many go to the FMA pipe.
-template <int D>
-struct Poly {
-    static constexpr int kOf4 = 1;
-};
+// One pair of weights in so many goes to the FMA pipe. A pair takes it as long there (14 cycles of a scheduler, and 8 of the ALU) as on the special
+// function unit (16), so the share that pays is small: none 494, an eighth 482, a quarter 484, three eighths 537 us (8192 tokens, causal).
+constexpr int kPolyShare = 8;
 
 template <int REGS>
 __device__ __forceinline__ void MoreRegisters()
@@ -609,7 +607,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                     for (int e = 0; e < 16; e++) {
                         const uint64_t y = Fma2(Both(x[c + 2 * e], x[c + 2 * e + 1]), factor2, from2);
                         float2 u;
-                        if (e % 4 < Poly<D>::kOf4) {
+                        if (e % kPolyShare == 0) {
                             u = Exp2Poly<kBf16>(y);
                         } else {
                             u = Apart(y);
