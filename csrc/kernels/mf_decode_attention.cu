@@ -34,7 +34,7 @@ using namespace mf::attn;
 using mf::sm100::GridDependency;
 
 constexpr int kThreads = 128;
-constexpr int kCtasPerSm = 2;
+constexpr int kMostCtasPerSm = 3;
 constexpr int kWarps = 4;
 constexpr int kWholeKeys = 256;
 constexpr int kRowCost = 3;        // tiles that beginning and ending a row takes as long as
@@ -49,7 +49,9 @@ struct Cfg {
     static constexpr int kBlocks = kRow <= 128 ? 2 : 1;  // of 16 keys: narrow rows are worked on two by two
     static constexpr int kWarpKeys = 16 * kBlocks, kTileKeys = kWarps * kWarpKeys, kWholeTiles = kWholeKeys / kTileKeys;
     static constexpr uint32_t kStage = kWarpKeys * kRow * 2;  // keys and values of a warp's part of a tile
-    static constexpr int kStages = 24576 / kStage;
+    // Where a block of keys takes many instructions for its bytes (8-bit ones), three CTAs per SM with two stages hide more than two with three.
+    static constexpr int kCtasPerSm = sizeof(C) == 1 && NT == 1 ? 3 : 2;
+    static constexpr int kStages = (kCtasPerSm == 3 ? 16384 : 24576) / kStage;
     static constexpr uint32_t kRing = kStages * kStage;
     static constexpr int kRows = 8 * NT;
     static constexpr int kJoinRow = D + 4;  // floats from head to head: the lanes of a store fall into 32 banks
@@ -123,7 +125,7 @@ __device__ __forceinline__ float *Partial(float *ws, int cta, int which)
 
 // NT: query heads of a row of the line, in eights.
 template <typename Q, typename C, int D, int NT>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) mf_decode_attention_kernel(const __grid_constant__ mf_decode_attention_args_t a)
+__global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode_attention_kernel(const __grid_constant__ mf_decode_attention_args_t a)
 {
     using X = Cfg<C, D, NT>;
     using T = typename Operand<Q, C>::type;
@@ -696,7 +698,7 @@ int Ctas(int B, int kvHeads, int group, long long capacity)
 {
     const int sms = mf_k_sm_count(), rows = 8 * Eights(group);
     const long long tiles = (long long)B * kvHeads * ((group + rows - 1) / rows) * ((capacity + 63) / 64),  // tiles have 64 keys or more
-                    most = (long long)kCtasPerSm * (sms > 0 ? sms : 1);
+                    most = (long long)kMostCtasPerSm * (sms > 0 ? sms : 1);
     return (int)(tiles < most ? (tiles > 1 ? tiles : 1) : most);
 }
 
@@ -707,6 +709,9 @@ int Launch(const mf_decode_attention_args_t &a, int ctas, cudaStream_t stream)
 {
     using X = Cfg<C, D, NT>;
     constexpr uint32_t kSmem = X::kSmem;
+    static_assert(X::kCtasPerSm <= kMostCtasPerSm, "the workspace has room for the partial results of that many");
+    const int room = X::kCtasPerSm * mf_k_sm_count();
+    ctas = ctas < room ? ctas : room;
     if (!mf::AllowSmem<mf_decode_attention_kernel<Q, C, D, NT>>(kSmem)) {
         return MF_K_LAUNCH_FAILED;
     }

@@ -177,6 +177,10 @@ __device__ __forceinline__ int ClaimedCta(const uint4 *answer)
     return x;
 }
 
+// A row that is computed again key by key (AttendRow) holds its CTA up for as long as that takes, 2.5 seconds for a million keys, so the waits in this kernel
+// have a minute.
+__device__ __forceinline__ bool Wait(uint64_t *bar, uint32_t parity, volatile int *abortFlag) { return MbarWaitWarp(bar, parity, abortFlag, 60000000000ull); }
+
 // Sequence b's query rows and keys, as far as there are tokens.
 __device__ __forceinline__ void Extent(const mf_prefill_attention_args_t &a, int b, Work &w)
 {
@@ -276,7 +280,7 @@ struct Worker {
     int k{0};
     __device__ __forceinline__ bool Next(Shared<D> &s, volatile int *abortFlag, Work &w)
     {
-        if (!MbarWaitWarp(&s.workFull[k & 1], (k >> 1) & 1, abortFlag)) {
+        if (!Wait(&s.workFull[k & 1], (k >> 1) & 1, abortFlag)) {
             return false;
         }
         w = s.work[k & 1];
@@ -358,7 +362,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                         s.work[k & 1] = w;
                         MbarArrive(&s.workFull[k & 1]);
                     }
-                    if (end || !MbarWaitWarp(&s.workEmpty[k & 1], (k >> 1) & 1, abortFlag)) {  // so the other place is free, too
+                    if (end || !Wait(&s.workEmpty[k & 1], (k >> 1) & 1, abortFlag)) {  // so the other place is free, too
                         break;
                     }
                     k++;
@@ -368,7 +372,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                     ClaimCta(&s.claim, &s.claimed);
                 }
                 int own = 0;  // the answer is waited for even if the CTA gives up: it is written to its shared memory
-                if (!MbarWaitWarp(&s.claimed, claims & 1, &own)) {
+                if (!Wait(&s.claimed, claims & 1, &own)) {
                     *abortFlag = 1;
                     break;
                 }
@@ -388,7 +392,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                     continue;
                 }
                 const bool two = w.t0 + half < w.rows;
-                ok = MbarWaitWarp(&s.qEmpty, qPh ^ 1, abortFlag);
+                ok = Wait(&s.qEmpty, qPh ^ 1, abortFlag);
                 if (!ok) {
                     break;
                 }
@@ -403,7 +407,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                 qOpen = true;
                 qPh ^= 1;
                 for (int i = 0; i < 2 * w.n; i++) {
-                    ok = MbarWaitWarp(&s.kvEmpty[st], ph ^ 1, abortFlag);
+                    ok = Wait(&s.kvEmpty[st], ph ^ 1, abortFlag);
                     if (!ok) {
                         break;
                     }
@@ -469,14 +473,14 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                 if (n == 0) {
                     continue;
                 }
-                ok = MbarWaitWarp(&s.qFull, qPh, abortFlag);
+                ok = Wait(&s.qFull, qPh, abortFlag);
                 qPh ^= 1;
                 if (__any_sync(~0u, i == 1 && w.t0 + half >= w.rows)) {  // no second tile: its share of the stages is given back at once
                     if (ok && elected) {
                         MbarArrive(&s.qEmpty);
                     }
                     for (int j = 0; ok && j < 2 * n; j++) {
-                        ok = MbarWaitWarp(&s.kvFull[st], ph, abortFlag);
+                        ok = Wait(&s.kvFull[st], ph, abortFlag);
                         if (ok && elected) {
                             MbarArrive(&s.kvEmpty[st]);
                         }
@@ -484,7 +488,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                     }
                     continue;
                 }
-                ok = ok && MbarWaitWarp(&s.kvFull[st], ph, abortFlag);
+                ok = ok && Wait(&s.kvFull[st], ph, abortFlag);
                 if (!ok) {
                     break;
                 }
@@ -506,8 +510,8 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                     if (next) {
                         step();
                     }
-                    ok = MbarWaitWarp(&s.kvFull[v], vPh, abortFlag) && (!next || MbarWaitWarp(&s.kvFull[k], kPh, abortFlag)) &&
-                         MbarWaitWarp(&s.pFull[i], pPh, abortFlag);
+                    ok = Wait(&s.kvFull[v], vPh, abortFlag) && (!next || Wait(&s.kvFull[k], kPh, abortFlag)) &&
+                         Wait(&s.pFull[i], pPh, abortFlag);
                     if (!ok) {
                         break;
                     }
@@ -515,7 +519,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                     if (elected) {
                         values(v, j > 0, 0, kEarly);
                     }
-                    ok = MbarWaitWarp(&s.pRest[i], pPh, abortFlag);
+                    ok = Wait(&s.pRest[i], pPh, abortFlag);
                     if (!ok) {
                         break;
                     }
@@ -651,7 +655,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
             top = -INFINITY;
             sum = 0;
             for (int j = 0; j < w.n; j++) {
-                if (!MbarWaitWarp(&s.sFull[i], sPh, abortFlag)) {
+                if (!Wait(&s.sFull[i], sPh, abortFlag)) {
                     ok = false;
                     break;
                 }
@@ -663,7 +667,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                     tile(std::true_type{}, j == 0, limit - j * kTile, most - j * kTile);
                 }
             }
-            if (!ok || (w.n > 0 && !MbarWaitWarp(&s.oFull[i], oPh, abortFlag))) {
+            if (!ok || (w.n > 0 && !Wait(&s.oFull[i], oPh, abortFlag))) {
                 break;
             }
             oPh ^= w.n > 0 ? 1 : 0;

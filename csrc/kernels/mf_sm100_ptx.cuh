@@ -78,9 +78,9 @@ __device__ __forceinline__ bool MbarWaitBounded(uint64_t *bar, uint32_t parity, 
 // The same by a whole warp, with one answer for all lanes. The warps that feed the tensor cores run their loops uniformly and let one
 // elected lane issue: descriptors and addresses then stay in uniform registers, which is where the instructions want them. In a
 // loop of one lane they were moved there operand by operand, and issuing a K block took longer than its MMAs.
-__device__ __forceinline__ bool MbarWaitWarp(uint64_t *bar, uint32_t parity, volatile int *abortFlag)
+__device__ __forceinline__ bool MbarWaitWarp(uint64_t *bar, uint32_t parity, volatile int *abortFlag, uint64_t limitNs = 2000000000ull)
 {
-    return __all_sync(0xffffffffu, MbarWaitBounded(bar, parity, abortFlag)) != 0;
+    return __all_sync(0xffffffffu, MbarWaitBounded(bar, parity, abortFlag, limitNs)) != 0;
 }
 // True in one lane of the (converged) warp.
 __device__ __forceinline__ bool ElectOne()

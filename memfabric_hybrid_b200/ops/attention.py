@@ -180,7 +180,7 @@ def decode_attention(q, k_pages, v_pages, table, lengths, *, rows=None, scale=No
 
     status: int32 tensor of one element, receives MF_DEV_ERR_BOUNDS (2) where a length reaches a page number that does not exist (its
     keys and values then count as zeros) or rows names no sequence (which then has no tokens)."""
-    no_gradient(q)
+    no_gradient(q, k_pages, v_pages)
     with_lse = lse is not None and lse is not False
     if lse is True or lse is False:
         lse = None
