@@ -2,7 +2,8 @@
 """Small, self-ending single-GPU cases for profiler captures: each runs ONE kernel of the library a few times on inputs that
 are larger than L2 (126 MB) where DRAM figures matter but hold at most a few GB on the device.
 
-    python benchmarks/profile_cases.py xcopy | shifted | peer | batch | gemm | gemm_2sm | gemm2 | gemm_fp32 | allreduce | epilogue | dispatch | moe_rank | reshard
+    python benchmarks/profile_cases.py xcopy | shifted | peer | batch | gemm | gemm_2sm | gemm2 | gemm_fp32 | allreduce | epilogue | dispatch | moe_rank | reshard |
+        prefill | decode | decode_e4m3 | compact
 
 `peer` needs two GPUs in ONE process (no second rank): GPU 0 pushes 256 MiB into GPU 1's memory over NVLink, so the link's byte
 counters (nvltx__bytes / nvlrx__bytes) can be read next to the kernel's duration.
@@ -272,6 +273,65 @@ def case_reshard():
     for _ in range(2):
         res = emulated_reshard(heap, plans, off)
         assert all(st == 0 for _, _, st in res)
+
+
+def case_prefill():
+    """One causal prompt of 4096 tokens, 32 heads on 8."""
+    import torch
+    from memfabric_hybrid_b200.ops.attention import prefill_attention
+
+    T = 4096
+    qkv = torch.randn(T, 48, 128, dtype=torch.bfloat16, device="cuda")
+    cu = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    for _ in range(3):
+        prefill_attention(qkv[:, :32], qkv[:, 32:40], qkv[:, 40:], cu)
+
+
+def _cached(dtype, seqs=64, length=2000, page=16):
+    import torch
+    from memfabric_hybrid_b200.ops.kv_cache import PagedKVCache
+
+    width = -(-length // page)
+    cache = PagedKVCache.allocate(1, seqs * width, page, 8, 128, seqs, width, dtype)
+    cache.data.copy_(torch.randn(cache.data.shape, dtype=torch.bfloat16, device="cuda").to(dtype))
+    cache.reserve(torch.arange(seqs, dtype=torch.int32, device="cuda"), torch.full((seqs,), length, dtype=torch.int32, device="cuda"), seqs * length)
+    return cache
+
+
+def case_decode(dtype=None):
+    """64 sequences of 2000 tokens, 32 heads on 8: 524 MB of bf16 keys and values."""
+    import torch
+
+    cache = _cached(dtype or torch.bfloat16)
+    scales = {n: torch.ones(8, device="cuda") for n in ("k_scale", "v_scale")} if dtype is not None else {}
+    q = torch.randn(64, 32, 128, dtype=torch.bfloat16, device="cuda")
+    for _ in range(3):
+        cache.decode(0, q, **scales)
+    assert cache.check_status() == 0
+
+
+def case_decode_e4m3():
+    import torch
+
+    case_decode(torch.float8_e4m3fn)
+
+
+def case_compact():
+    """A cache of 16 layers, every other sequence of which is dropped: 268 MB of pages move."""
+    import torch
+    from memfabric_hybrid_b200.ops.kv_cache import PagedKVCache
+
+    cache = PagedKVCache.allocate(16, 2048, 16, 4, 128, 64, 32)
+    seqs = torch.arange(64, dtype=torch.int32, device="cuda")
+    cache.reserve(seqs, torch.full((64,), 512, dtype=torch.int32, device="cuda"), 64 * 512)
+    for _ in range(3):
+        cache.free(seqs[::2].contiguous())
+        cache.compact()
+        cache.reserve(seqs[::2].contiguous(), torch.full((32,), 512, dtype=torch.int32, device="cuda"), 32 * 512)
+        cache.free(seqs[1::2].contiguous())
+        cache.compact()
+        cache.reserve(seqs[1::2].contiguous(), torch.full((32,), 512, dtype=torch.int32, device="cuda"), 32 * 512)
+    assert cache.check_status() == 0
 
 
 if __name__ == "__main__":

@@ -181,13 +181,14 @@ __device__ __forceinline__ int ClaimedCta(const uint4 *answer)
 // have a minute.
 __device__ __forceinline__ bool Wait(uint64_t *bar, uint32_t parity, volatile int *abortFlag) { return MbarWaitWarp(bar, parity, abortFlag, 60000000000ull); }
 
-// Sequence b's query rows and keys, as far as there are tokens.
+// Sequence b's query rows and keys, as far as there are tokens; none where the offsets descend or begin outside.
 __device__ __forceinline__ void Extent(const mf_prefill_attention_args_t &a, int b, Work &w)
 {
+    auto within = [](int first, int next, int all) { return first < 0 || first >= all ? 0 : min(max(next, first), all) - first; };
     w.q0 = a.cuQ[b];
-    w.rows = w.q0 < 0 ? 0 : min(a.cuQ[b + 1], a.tokensQ) - w.q0;
+    w.rows = within(w.q0, a.cuQ[b + 1], a.tokensQ);
     w.k0 = a.cuK[b];
-    w.keys = w.k0 < 0 ? 0 : min(a.cuK[b + 1], a.tokensK) - w.k0;
+    w.keys = within(w.k0, a.cuK[b + 1], a.tokensK);
 }
 
 // Row tiles of sequence b have numbers from cuQ[b] / tokens + b on: enough for its rows wherever they begin, some numbers stay empty. Taken from

@@ -1,5 +1,5 @@
-"""Torch-facing wrappers of the fused kernels: allreduce (+residual+RMSNorm), MoE dispatch / grouped FP8 GEMM / combine, weight
-reshard, and `smoke_all`, a quick self-check that launches every kernel of the library once on small inputs."""
+"""Torch-facing wrappers of the fused kernels: allreduce (+residual+RMSNorm), MoE dispatch / grouped FP8 GEMM / combine, attention over
+prompts and over a paged key-value cache, weight reshard, and `smoke_all`, a quick self-check that launches every kernel of the library once on small inputs."""
 from __future__ import annotations
 
 
@@ -7,7 +7,8 @@ def smoke_all(verbose: bool = False) -> dict:
     """Launches every kernel family on `cuda:<current>` with small inputs and checks each result against its PyTorch oracle:
     single copies through both copy kernels, the inline, the table and the bulk batch copy, all-reduce + RMSNorm (one-shot and
     two-shot, four emulated ranks; one real rank), MoE dispatch → block-scaled grouped GEMMs → combine (two emulated ranks; one
-    real rank), the fp32-scale grouped GEMM and the row quantiser, and the weight reshard (bf16 and fp8, four emulated ranks).
+    real rank), the fp32-scale grouped GEMM and the row quantiser, the weight reshard (bf16 and fp8, four emulated ranks), and a step of a
+    paged key-value cache: prompts attended and written, forked, decoded, compacted (bf16 and e4m3).
     Returns {name: True}; raises on the first mismatch."""
     import socket
 
@@ -18,7 +19,9 @@ def smoke_all(verbose: bool = False) -> dict:
     from ..models import LlamaConfig, param_specs
     from ..parallel.heap import EmulatedHeap, SymmetricHeap
     from . import fp8_gemm as F
+    from . import attention as A
     from .allreduce import AllReduceRMSNorm, emulated_allreduce, reference
+    from .kv_cache import PagedKVCache
     from .moe import EmulatedMoE, FusedMoE, moe_reference, route
     from .reshard import ReshardPlan, emulated_reshard, reference_reshard
 
@@ -180,4 +183,28 @@ def smoke_all(verbose: bool = False) -> dict:
                 else:
                     assert torch.equal(dst[e.dst_off:e.dst_off + 2 * nel].view(torch.bfloat16), refd[e.spec.name].reshape(-1))
         mark("reshard_fp8" if fp8 else "reshard_bf16")
+    # ---- a paged cache: two prompts, a candidate of the first, a decode step of all three before and after compaction
+    def close(out, ref):
+        torch.testing.assert_close(out.double(), ref, atol=2e-2, rtol=2e-2)
+
+    heads, kv, dim, lens = 8, 2, 128, [300, 77]
+    cu = torch.tensor([0, 300, 377], dtype=torch.int32, device=dev)
+    x = torch.randn(377, heads + 2 * kv, dim, generator=g, device=dev).to(torch.bfloat16)
+    q, k, v = x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:]
+    close(A.prefill_attention(q, k, v, cu), A.prefill_attention_reference(q, k, v, cu)[0])
+    mark("prefill_attention")
+    for dtype in (torch.bfloat16, torch.float8_e4m3fn):
+        scales = {n: torch.full((kv,), 0.01, device=dev) for n in ("k_scale", "v_scale")} if dtype == torch.float8_e4m3fn else {}
+        cache = PagedKVCache.allocate(1, 64, 16, kv, dim, 4, 32, dtype)
+        number = {n: torch.tensor(n, dtype=torch.int32, device=dev) for n in ((0,), (2,), (0, 1), (0, 1, 2), (1, 1, 1), tuple(lens))}
+        cache.write(0, k, v, cache.reserve(number[0, 1], number[tuple(lens)], 377), **scales)
+        cache.fork(number[0,], number[2,])
+        cache.write(0, k[:3], v[:3], cache.reserve(number[0, 1, 2], number[1, 1, 1], 3), **scales)
+        ref = A.decode_attention_reference(q[:3], cache.k_pages(0), cache.v_pages(0), cache.table, cache.lengths, **scales)[0]
+        close(cache.decode(0, q[:3], **scales), ref)
+        cache.free(number[0,])
+        cache.compact()
+        close(cache.decode(0, q[1:3], number[0, 1, 2][1:], **scales), ref[1:])
+        assert cache.check_status() == 0
+        mark("kv_cache_" + ("bf16" if dtype == torch.bfloat16 else "e4m3"))
     return done

@@ -115,8 +115,11 @@ def _check_result(out, like_shape, like_dtype, lse, lse_shape):
     if out is not None:
         if out.shape != like_shape or out.dtype != like_dtype:
             raise ValueError(f"out must be {tuple(like_shape)} {like_dtype}")
-        if (out.shape[1] > 1 and out.stride(1) < out.shape[2]) or (out.shape[0] > 1 and out.stride(0) < out.shape[1] * out.stride(1)):
-            raise ValueError("out must not overlap itself")
+        taken = out.shape[2]
+        for step, n in sorted((out.stride(d), out.shape[d]) for d in (0, 1) if out.shape[d] > 1):
+            if step < taken:
+                raise ValueError("out must not overlap itself")
+            taken = step * n
     if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != lse_shape or not lse.is_contiguous()):
         raise ValueError(f"lse must be a contiguous fp32 tensor {lse_shape}")
 

@@ -410,3 +410,76 @@ def test_prefill_strides_scale_and_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, A.prefill_attention(q, k, v, cu, scale=0.3))
+
+
+@pytest.mark.parametrize("count,most", [(64, 300), (65, 300), (200, 40), (7, 1500)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prefill_many_sequences_of_random_lengths(count, most, causal):
+    """Every row tile of every sequence is done once, however the work is dealt out: few sequences are ranked by what they take, many are not."""
+    import random
+
+    import torch
+
+    r = random.Random(count)
+    rows = [r.choice([0, 1, r.randint(1, most)]) for _ in range(count)]
+    keys = [r.choice([n, n, 0, n + r.randint(0, most), max(0, n - 40)]) for n in rows]
+    _prefill_case(rows, keys, 6, 2, 64, torch.bfloat16, causal)
+
+
+@pytest.mark.parametrize("heads,kv", [(12, 1), (40, 4), (100, 1), (14, 2), (11, 1)])
+def test_prefill_heads_packed_into_tiles_that_they_do_not_fill(heads, kv):
+    import torch
+
+    _prefill_case([1, 130, 37, 300], [1, 130, 200, 300], heads, kv, 128, torch.float16, True)
+
+
+def test_prefill_head_major_tensors():
+    """Heads before tokens in memory: strides in the other order."""
+    import torch
+
+    from memfabric_hybrid_b200.ops import attention as A
+
+    cu = torch.tensor([0, 150, 310], dtype=torch.int32, device="cuda")
+    q, k, v = (_q((n, 310, 64), torch.bfloat16, s).transpose(0, 1) for n, s in ((6, 1), (2, 2), (2, 3)))
+    want = A.prefill_attention(q.contiguous(), k.contiguous(), v.contiguous(), cu)
+    assert torch.equal(A.prefill_attention(q, k, v, cu), want)
+    out = torch.empty(6, 310, 64, dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+    assert torch.equal(A.prefill_attention(q, k, v, cu, out=out), want)
+
+
+def test_prefill_of_nothing():
+    import torch
+
+    from memfabric_hybrid_b200.ops import attention as A
+
+    cu = torch.zeros(1, dtype=torch.int32, device="cuda")
+    x = _q((5, 4, 64), torch.bfloat16)
+    out = torch.full_like(x, 2.0)
+    assert torch.equal(A.prefill_attention(x, x, x, cu, out=out), torch.full_like(x, 2.0))
+    none = x[:0]
+    assert A.prefill_attention(none, x, x, torch.zeros(3, dtype=torch.int32, device="cuda")).shape == (0, 4, 64)
+    out, lse = A.prefill_attention(x, none, none, torch.tensor([0, 5], dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"), lse=True)
+    assert bool((out == 0).all()) and bool((lse == -INF).all())
+    d = torch.zeros(1, 2, 4, 16, 64, dtype=torch.bfloat16, device="cuda")
+    assert A.decode_attention(x[:0], d[:, 0], d[:, 1], torch.zeros(0, 3, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda")).shape == (0, 4, 64)
+    one = A.decode_attention(x, d[:, 0], d[:, 1], torch.zeros(5, 0, dtype=torch.int32, device="cuda"), torch.full((5,), 9, dtype=torch.int32, device="cuda"))
+    assert bool((one == 0).all())
+
+
+def test_offsets_that_leave_the_tensors_are_cut_off():
+    """cu_q and cu_k that say more than there are tokens, or begin below zero: nothing outside is read or written."""
+    import torch
+
+    from memfabric_hybrid_b200.ops import attention as A
+
+    q, k, v = _q((100, 4, 64), torch.bfloat16, 1), _q((90, 2, 64), torch.bfloat16, 2), _q((90, 2, 64), torch.bfloat16, 3)
+    room = torch.full((140, 4, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    cu = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    A.prefill_attention(q, k, v, cu(0, 60, 1000), cu(0, 60, 2 ** 31 - 1), out=room[20:120])
+    want = A.prefill_attention(q, k, v, cu(0, 60, 100), cu(0, 60, 90))
+    assert torch.equal(room[20:120], want)
+    for bad in (cu(-8, 60, 100), cu(2 ** 31 - 1, -5, 7), cu(100, 60, 0)):
+        A.prefill_attention(q, k, v, bad, cu(0, 60, 90), out=room[20:120])
+        A.prefill_attention(q, k, v, cu(0, 60, 100), bad, out=room[20:120])
+    torch.cuda.synchronize()
+    assert bool((room[:20] == 5).all() and (room[120:] == 5).all())

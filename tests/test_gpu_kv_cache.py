@@ -292,3 +292,45 @@ def test_serving_loop(dtype):
     cache.compact()
     step([0, 4, 3], [1] * 3, False)
     assert cache.check_status() == 0
+
+
+def test_cache_in_pooled_memory_whose_pages_are_moved_by_batch_copies(port):
+    """Two caches in one rank's pooled HBM, as a prefill and a decode instance have them: a sequence's blocks go from one to the other by one batch
+    call, and are decoded there."""
+    import torch
+
+    from memfabric_hybrid_b200 import bm
+    from memfabric_hybrid_b200.ops.kv_cache import PagedKVCache
+    from memfabric_hybrid_b200.parallel.pool import open_pool
+    from memfabric_hybrid_b200.utils.tensors import device_tensor_from_gva
+
+    torch.cuda.set_device(0)
+    pool = open_pool(0, 1, 0, 64 << 20, store_url=f"tcp://127.0.0.1:{port}")
+    try:
+        layers, pages, page, kv, dim = 3, 40, 16, 2, 64
+        shape = (layers, pages, 2, kv, page, dim)
+        nbytes = 2 * layers * pages * 2 * kv * page * dim
+        caches = []
+        for i in range(2):
+            data = device_tensor_from_gva(pool.hbm() + i * (32 << 20), nbytes, torch.bfloat16).view(shape)
+            data.zero_()
+            caches.append(PagedKVCache(data, torch.full((3, 8), -1, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda"),
+                                       torch.zeros(pages, dtype=torch.int32, device="cuda")))
+        there, here = caches
+        g = torch.Generator(device="cuda").manual_seed(3)
+        slots = there.reserve(_ints([2, 1]), _ints([19, 100]), 119)
+        for layer in range(layers):
+            there.write(layer, *(torch.randn(119, kv, dim, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2)), slots)
+        here.reserve(_ints([0, 1]), _ints([40, 100]), 140)
+        q = torch.randn(1, 8, dim, generator=g, device="cuda").to(torch.bfloat16)
+        want = [there.decode(layer, q, _ints([1])) for layer in range(layers)]
+        torch.cuda.synchronize()
+        moves = [(there.block(layer, a), here.block(layer, b)) for layer in range(layers) for a, b in zip(there.table[1, :7].tolist(), here.table[1, :7].tolist())]
+        assert pool.handle.copy_data_batch([a for (a, _), _ in moves], [b for _, (b, _) in moves], [n for (_, n), _ in moves], len(moves), bm.BmCopyType.G2G, 0) == 0
+        for layer in range(layers):
+            assert torch.equal(here.decode(layer, q, _ints([1])), want[layer])
+        assert there.check_status() == 0 and here.check_status() == 0
+        del there, here, caches, data, want
+    finally:
+        torch.cuda.synchronize()
+        pool.close()
