@@ -741,8 +741,8 @@ int LaunchDim(const mf_decode_attention_args_t &a, int D, int ctas, cudaStream_t
 
 extern "C" size_t mf_k_decode_attention_workspace(int B, int kvHeads, int group, int D, long long capacity)
 {
-    if (B <= 0 || kvHeads <= 0 || group <= 0 || (D != 64 && D != 128) || capacity < 0) {
-        return 0;
+    if (B <= 0 || kvHeads <= 0 || group <= 0 || (D != 64 && D != 128) || capacity <= kWholeKeys) {
+        return 0;  // no row is cut
     }
     const int ctas = Ctas(B, kvHeads, group, capacity);
     return PartialBytes(ctas, group, D) + (size_t)ctas * 2 * sizeof(int2);
@@ -768,10 +768,13 @@ extern "C" int mf_k_decode_attention(const mf_decode_attention_args_t *args, int
     a.pageMagic = a.pageSize == 1 ? 0 : (uint32_t)(((1ull << (32 + a.pageShift)) + a.pageSize - 1) / a.pageSize);
     const long long capacity = (long long)a.tableWidth * a.pageSize;
     const int ctas = Ctas(a.B, a.kvHeads, a.group, capacity);
-    if (a.workspace == nullptr) {
+    if (capacity <= kWholeKeys) {
+        a.workspace = a.marks = nullptr;
+    } else if (a.workspace == nullptr) {
         return MF_K_INVALID;
+    } else {
+        a.marks = (unsigned char *)a.workspace + PartialBytes(ctas, a.group, D);
     }
-    a.marks = (unsigned char *)a.workspace + PartialBytes(ctas, a.group, D);
     if (qType == MF_K_BF16 && cacheType == MF_K_BF16) {
         return LaunchDim<__nv_bfloat16, __nv_bfloat16>(a, D, ctas, (cudaStream_t)stream);
     }

@@ -264,7 +264,7 @@ typedef struct {
     void *out;
     float *lse;
     int *status;
-    void *workspace;  // mf_k_decode_attention_workspace() bytes of this call's own
+    void *workspace;  // mf_k_decode_attention_workspace() bytes of this call's own (NULL if that says 0)
     void *marks;      // set by the launcher
     long long qStride[2];
     long long outStride[2];

@@ -200,13 +200,13 @@ def decode_attention(q, k_pages, v_pages, table, lengths, *, rows=None, scale=No
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         if with_lse and lse is None:
             lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-        ws = table.new_empty(words)
+        ws = table.new_empty(words) if words else None
         at = q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr()
         if (at[0] | at[1] | at[2] | at[3]) & 15:
             raise ValueError(_misaligned)
         rc = native.run(*at, table.data_ptr(), lengths.data_ptr(), 0 if rows is None else rows.data_ptr(), 0 if k_scale is None else k_scale.data_ptr(),
                         0 if v_scale is None else v_scale.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if status is None else status.data_ptr(),
-                        ws.data_ptr(), factor, current_stream_handle())
+                        0 if ws is None else ws.data_ptr(), factor, current_stream_handle())
     if rc != 0:
         raise RuntimeError(f"decode_attention launch failed ({rc})")
     return (out, lse) if with_lse else out
