@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode
         const uint32_t at = ring + take * X::kStage;
         if (key0 < cur.length) {
             // A block behind the end of the sequence holds what was there before: its scores are masked, its values left alone.
-            const int blocks = kBlocks == 1 || key0 + 16 >= cur.length ? 1 : kBlocks;
+            const int blocks = kBlocks == 1 ? 1 : min(kBlocks, (cur.length - key0 + 15) / 16);
             float x[kBlocks][NT][4];  // [key quad, quad + 8][head 2 pos, 2 pos + 1]
             bool grown = false;
 #pragma unroll
