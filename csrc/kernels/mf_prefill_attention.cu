@@ -12,9 +12,10 @@
 //                    the tensor core works for the other: O += P V of a key tile and S of the next one are issued together, the first reads
 //                    the P that the second overwrites, and the tensor core takes them in order.
 //   warp 9           TMA: both Q tiles, then keys and values in turn through a ring of stages.
+//   warp 10          takes the CTA's next two row tiles from the work that is left, while the present ones are computed.
 //
-// The reference m only follows the maximum where a weight would pass 2^8 (fp16: 2^14); then the row's O is scaled in TMEM. That is rare, so no warps are kept for it. The S barrier of a key tile stands for the
-// completion of all MMAs before it, so O is at rest when its S arrives.
+// The reference m only follows the maximum where a weight would pass 2^8 (fp16: 2^14); then the row's O is scaled in TMEM. That is rare, so no
+// warps are kept for it. The S barrier of a key tile stands for the completion of all MMAs before it, so O is at rest when its S arrives.
 //
 // p is rounded to the operands' type for the second product (the tensor core wants one type for both); the sum is taken before
 // that, all sums and O are fp32. A masked key counts 0 * v in a tile product, which is not 0 where v is infinite or NaN: a row whose result is not finite
@@ -36,9 +37,10 @@ using namespace mf::sm100;
 constexpr int kTile = 128;  // rows of a tile, keys of a tile
 constexpr int kThreads = 384;
 constexpr uint32_t kHalf = kTile * 128;  // bytes of 64 columns of a tile
-constexpr int kEarly = 96;               // keys whose P is handed over while the others are still computed
-// Registers of a softmax thread, which holds a row of S, and of the others: 256 * 200 + 128 * 96 of the 384 * 168 of the launch.
-constexpr int kSoftmaxRegs = 200, kOtherRegs = 96;
+constexpr int kEarly = 64;  // keys whose P is handed over while the others are still computed
+// Registers of a softmax thread, which holds a row of S, and of the others: 256 * 216 + 128 * 72 = the 384 * 168 of the launch. 16384 tokens, long loops:
+// 200 and 96 1935 us, 216 and 72 1897, 232 and 40 1937.
+constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 
 // What the scheduler warp says about a CTA's next two row tiles.
 struct Work {
@@ -140,9 +142,13 @@ __device__ __forceinline__ float2 Exp2Poly(uint64_t x2)
     return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(r.x) << 23)), __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23)));
 }
 
-// One pair of weights in so many goes to the FMA pipe. A pair takes it as long there (14 cycles of a scheduler, and 8 of the ALU) as on the special
-// function unit (16), so the share that pays is small: none 494, an eighth 482, a quarter 484, three eighths 537 us (8192 tokens, causal).
-constexpr int kPolyShare = 8;
+// One pair of weights in so many goes to the FMA pipe. A pair takes it as long there (14 cycles of a scheduler, and 8 of the ALU; 16 with degree 4) as on
+// the special function unit (16), so the share that pays is small. 8192 tokens, bf16: none 494, an eighth 482, three eighths 537 us; with the
+// present split of registers an eighth 513, a quarter 506 us (long loops). fp16, 12 prompts: none 72, an eighth 73, a quarter 76 us.
+template <bool BF16>
+struct Poly {
+    static constexpr int kShare = BF16 ? 4 : 8;
+};
 
 template <int REGS>
 __device__ __forceinline__ void MoreRegisters()
@@ -308,10 +314,10 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
 
     if (threadIdx.x == 0) {
         MbarInit(&s.qFull, 1);
-        MbarInit(&s.qEmpty, 2);
+        MbarInit(&s.qEmpty, 1);
         for (int i = 0; i < X::kStages; i++) {
             MbarInit(&s.kvFull[i], 1);
-            MbarInit(&s.kvEmpty[i], 2);
+            MbarInit(&s.kvEmpty[i], 1);
         }
         for (int i = 0; i < 2; i++) {
             MbarInit(&s.sFull[i], 1);
@@ -319,7 +325,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
             MbarInit(&s.pRest[i], 4);
             MbarInit(&s.oFull[i], 1);
             MbarInit(&s.workFull[i], 1);
-            MbarInit(&s.workEmpty[i], 11);
+            MbarInit(&s.workEmpty[i], 10);
         }
         MbarInit(&s.claimed, 1);
         s.abortFlag = 0;
@@ -434,34 +440,34 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                     MbarWaitBounded(&s.kvFull[i % X::kStages], (uint32_t)(i / X::kStages) & 1, &own);
                 }
             }
-        } else {
-            // ------------------------------------------------------------------ MMA issuers, one for each tile
+        } else if (warp == 8) {
+            // ------------------------------------------------------------------ MMA issuer
             // Everything that the loops and operands go by comes out of a warp reduction: the compiler then knows that it is the same in all lanes and
-            // keeps descriptors in uniform registers.
+            // keeps descriptors in uniform registers. One warp for both tiles, so that the S of one is complete before that of the other is begun: issued by
+            // a warp for each, they took turns and were both late (chunks of prompts 154 -> 147 us, 16384 tokens 1963 -> 1935).
             const bool elected = ElectOne();
-            const int i = __reduce_max_sync(~0u, warp == 8 ? 0 : 1);
-            const uint32_t base = __reduce_or_sync(~0u, tmem), sAt = base + i * kTile, oAt = base + kO + i * D;
-            const uint64_t qDesc = SmemDescSw128(SmemAddr(s.q[0])) + i * (X::kTileBytes >> 4), kDesc = SmemDescSw128(SmemAddr(s.kv[0])),
+            const uint32_t base = __reduce_or_sync(~0u, tmem);
+            const uint64_t qDesc = SmemDescSw128(SmemAddr(s.q[0])), kDesc = SmemDescSw128(SmemAddr(s.kv[0])),
                            vDesc = SmemDescSw128Transposed(SmemAddr(s.kv[0]), kHalf);
             constexpr uint32_t iS = InstrDescF16(kTile, kTile, kBf16, false), iO = InstrDescF16(kTile, D, kBf16, true);
-            auto scores = [&](uint32_t stage) {
-                const uint64_t k0 = kDesc + stage * (X::kTileBytes >> 4);
+            auto scores = [&](int i, uint32_t stage) {  // S of tile i
+                const uint64_t k0 = kDesc + stage * (X::kTileBytes >> 4), q0 = qDesc + i * (X::kTileBytes >> 4);
 #pragma unroll
                 for (int k = 0; k < D / 16; k++) {
                     const uint32_t off = (k / 4) * (kHalf >> 4) + (k % 4) * 2;
-                    MmaF16(sAt, qDesc + off, k0 + off, iS, k > 0);
+                    MmaF16(base + i * kTile, q0 + off, k0 + off, iS, k > 0);
                 }
             };
-            auto values = [&](uint32_t stage, bool more, int k0, int k1) {  // of the keys [k0, k1)
+            auto values = [&](int i, uint32_t stage, bool more, int k0, int k1) {  // O of tile i, keys [k0, k1)
                 const uint64_t v0 = vDesc + stage * (X::kTileBytes >> 4);
 #pragma unroll
                 for (int k = k0 / 16; k < k1 / 16; k++) {
-                    MmaF16Tmem(oAt, sAt + k * 8, v0 + k * 128, iO, more || k > 0);
+                    MmaF16Tmem(base + kO + i * D, base + i * kTile + k * 8, v0 + k * 128, iO, more || k > 0);
                 }
             };
             Worker<D> worker;
             Work w;
-            uint32_t st = 0, ph = 0, qPh = 0, pPh = 0;
+            uint32_t st = 0, ph = 0, qPh = 0, pPh[2] = {0, 0};
             auto step = [&]() {
                 if (++st == X::kStages) {
                     st = 0;
@@ -470,40 +476,30 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
             };
             bool ok = true;
             while (ok && __any_sync(~0u, worker.Next(s, abortFlag, w))) {
-                const int n = __reduce_max_sync(~0u, w.n);
+                const int n = __reduce_max_sync(~0u, w.n), both = __reduce_max_sync(~0u, w.t0 + half < w.rows ? 2 : 1);
                 if (n == 0) {
                     continue;
                 }
-                ok = Wait(&s.qFull, qPh, abortFlag);
+                ok = Wait(&s.qFull, qPh, abortFlag) && Wait(&s.kvFull[st], ph, abortFlag);
                 qPh ^= 1;
-                if (__any_sync(~0u, i == 1 && w.t0 + half >= w.rows)) {  // no second tile: its share of the stages is given back at once
-                    if (ok && elected) {
-                        MbarArrive(&s.qEmpty);
-                    }
-                    for (int j = 0; ok && j < 2 * n; j++) {
-                        ok = Wait(&s.kvFull[st], ph, abortFlag);
-                        if (ok && elected) {
-                            MbarArrive(&s.kvEmpty[st]);
-                        }
-                        step();
-                    }
-                    continue;
-                }
-                ok = ok && Wait(&s.kvFull[st], ph, abortFlag);
                 if (!ok) {
                     break;
                 }
                 TcFenceAfter();
                 if (elected) {
-                    scores(st);
-                    MmaCommit(&s.sFull[i]);
+                    scores(0, st);
+                    MmaCommit(&s.sFull[0]);
+                    if (both == 2) {
+                        scores(1, st);
+                        MmaCommit(&s.sFull[1]);
+                    }
                     MmaCommit(&s.kvEmpty[st]);
                     if (n == 1) {
                         MmaCommit(&s.qEmpty);
                     }
                 }
                 step();
-                for (int j = 0; j < n; j++) {
+                for (int j = 0; ok && j < n; j++) {
                     const uint32_t v = st, vPh = ph;
                     step();
                     const uint32_t k = st, kPh = ph;
@@ -511,34 +507,44 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                     if (next) {
                         step();
                     }
-                    ok = Wait(&s.kvFull[v], vPh, abortFlag) && (!next || Wait(&s.kvFull[k], kPh, abortFlag)) &&
-                         Wait(&s.pFull[i], pPh, abortFlag);
-                    if (!ok) {
-                        break;
-                    }
-                    TcFenceAfter();
-                    if (elected) {
-                        values(v, j > 0, 0, kEarly);
-                    }
-                    ok = Wait(&s.pRest[i], pPh, abortFlag);
-                    if (!ok) {
-                        break;
-                    }
-                    pPh ^= 1;
-                    TcFenceAfter();
-                    if (elected) {
-                        values(v, true, kEarly, kTile);
-                        if (next) {
-                            scores(k);
-                            MmaCommit(&s.sFull[i]);
-                            MmaCommit(&s.kvEmpty[k]);
-                            if (j + 2 == n) {
-                                MmaCommit(&s.qEmpty);
-                            }
-                        } else {
-                            MmaCommit(&s.oFull[i]);
+                    ok = Wait(&s.kvFull[v], vPh, abortFlag) && (!next || Wait(&s.kvFull[k], kPh, abortFlag));
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        if (!ok || i >= both) {
+                            break;
                         }
-                        MmaCommit(&s.kvEmpty[v]);
+                        ok = Wait(&s.pFull[i], pPh[i], abortFlag);
+                        if (!ok) {
+                            break;
+                        }
+                        TcFenceAfter();
+                        if (elected) {
+                            values(i, v, j > 0, 0, kEarly);
+                        }
+                        ok = Wait(&s.pRest[i], pPh[i], abortFlag);
+                        if (!ok) {
+                            break;
+                        }
+                        pPh[i] ^= 1;
+                        TcFenceAfter();
+                        if (elected) {
+                            values(i, v, true, kEarly, kTile);
+                            if (next) {
+                                scores(i, k);
+                                MmaCommit(&s.sFull[i]);
+                                if (i + 1 == both) {
+                                    MmaCommit(&s.kvEmpty[k]);
+                                    if (j + 2 == n) {
+                                        MmaCommit(&s.qEmpty);
+                                    }
+                                }
+                            } else {
+                                MmaCommit(&s.oFull[i]);
+                            }
+                            if (i + 1 == both) {
+                                MmaCommit(&s.kvEmpty[v]);
+                            }
+                        }
                     }
                 }
             }
@@ -612,7 +618,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                     for (int e = 0; e < 16; e++) {
                         const uint64_t y = Fma2(Both(x[c + 2 * e], x[c + 2 * e + 1]), factor2, from2);
                         float2 u;
-                        if (e % kPolyShare == 0) {
+                        if (e % Poly<kBf16>::kShare == 0) {
                             u = Exp2Poly<kBf16>(y);
                         } else {
                             u = Apart(y);
