@@ -318,7 +318,7 @@ typedef struct {
 
 // Keys and values of `tokens` tokens, [tokens][kvHeads][dim] with strides {token, head} in elements, into the slots (page * pageSize + place in
 // the page) of one layer's pages, which `data` points to. Slots below 0 are left out, slots behind the last page too, with the status
-// set. One slot named twice gets one of the two rows. e4m3: x * (1 / scale of the head), rounded to nearest, saturated.
+// set. What a slot that is named twice holds is not defined. e4m3: x * (1 / scale of the head), rounded to nearest, saturated.
 typedef struct {
     const void *k;
     const void *v;

@@ -115,7 +115,8 @@ class PagedKVCache:
 
     def write(self, layer, k, v, slots, *, k_scale=None, v_scale=None, stream=None):
         """Puts keys and values [tokens, kv_heads, head_dim] (any strides, rows contiguous) of one layer into their slots (int64 [tokens], from
-        reserve(), or page * page_size + place). A slot below 0 leaves its token out; one behind the last page too, and sets the status.
+        reserve(), or page * page_size + place). A slot below 0 leaves its token out; one behind the last page too, and sets the status;
+        what one holds that is named twice is not defined.
         A float8_e4m3fn cache takes bf16 or fp16 and k_scale, v_scale fp32 [kv_heads]: it holds x * (1 / scale), rounded to nearest and
         saturated at 448; any other cache takes its own type."""
         key = (k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype, v.get_device(), slots.shape, slots.stride(), slots.dtype,

@@ -483,3 +483,59 @@ def test_offsets_that_leave_the_tensors_are_cut_off():
         A.prefill_attention(q, k, v, cu(0, 60, 100), bad, out=room[20:120])
     torch.cuda.synchronize()
     assert bool((room[:20] == 5).all() and (room[120:] == 5).all())
+
+
+def test_prefill_offsets_past_32_bits():
+    """Queries, keys, values and results of more than 2^32 bytes each: the last prompts of many against the same ones alone."""
+    import torch
+
+    from memfabric_hybrid_b200.ops import attention as A
+
+    count, n = 4200, 128
+    x = torch.empty(count * n, 32, 128, dtype=torch.bfloat16, device="cuda")  # 4.4 GB
+    last = slice((count - 3) * n, count * n)
+    x.zero_()
+    x[last].normal_(generator=torch.Generator(device="cuda").manual_seed(0))
+    cu = torch.arange(count + 1, device="cuda", dtype=torch.int32) * n
+    out = A.prefill_attention(x, x, x, cu)
+    assert torch.equal(out[last], A.prefill_attention(x[last], x[last], x[last], cu[:4].contiguous()))
+    assert bool((out[:n] == 0).all())
+
+
+def test_decode_thousands_of_sequences():
+    import torch
+
+    from memfabric_hybrid_b200.ops import attention as A
+
+    g = torch.Generator(device="cuda").manual_seed(2)
+    lens = torch.randint(0, 600, (5000,), generator=g, device="cuda", dtype=torch.int32)
+    data = torch.randn(997, 2, 2, 16, 64, generator=g, device="cuda").to(torch.bfloat16)
+    table = torch.randint(0, 997, (5000, 38), generator=g, device="cuda", dtype=torch.int32)
+    q = _q((5000, 8, 64), torch.bfloat16)
+    out = A.decode_attention(q, data[:, 0], data[:, 1], table, lens)
+    for rows in (slice(0, 7), slice(2500, 2507), slice(4993, 5000)):
+        ref, _ = A.decode_attention_reference(q[rows], data[:, 0], data[:, 1], table[rows], lens[rows])
+        mass, _ = A.decode_attention_reference(q[rows], data[:, 0], data[:, 1].abs(), table[rows], lens[rows])
+        _check(out[rows], ref, mass, torch.bfloat16, 64, 600, 40)
+
+
+def test_calls_on_several_streams_at_once():
+    """Prompts and decode steps that run side by side: nothing is shared between calls."""
+    import torch
+
+    from memfabric_hybrid_b200.ops import attention as A
+
+    x = _q((3000, 12, 128), torch.bfloat16)
+    cu = torch.tensor([0, 1100, 1101, 3000], dtype=torch.int32, device="cuda")
+    k, v, table, lens = _pool([5000, 900, 0, 333], 16, 2, 128, torch.bfloat16, spare=0)
+    q = _q((4, 8, 128), torch.bfloat16)
+    want_p, want_d = A.prefill_attention(x[:, :8], x[:, 8:10], x[:, 10:], cu), A.decode_attention(q, k, v, table, lens)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(4)], []
+    for turn in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((A.prefill_attention(x[:, :8], x[:, 8:10], x[:, 10:], cu) if (i + turn) % 2 else A.decode_attention(q, k, v, table, lens), (i + turn) % 2))
+    torch.cuda.synchronize()
+    for out, prompt in got:
+        assert torch.equal(out, want_p if prompt else want_d)
