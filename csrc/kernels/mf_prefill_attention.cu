@@ -217,69 +217,93 @@ __device__ __forceinline__ bool Numbered(const Params &p, int number, Work &w)
 }
 
 // The same for a few sequences, with the row tiles in order of the key tiles that they take, the most first: what is left at the end is small. How many
-// row tiles take m key tiles or more follows from a sequence's lengths; the m of a number is found by bisection. A lane has two sequences.
+// row tiles take m key tiles or more follows from a sequence's lengths; the m of a number is found by bisection. A lane has two sequences, the lengths of
+// which stay in registers, and divides by multiplying.
 constexpr int kRanked = 64;
-__device__ __forceinline__ bool Ranked(const Params &p, int number, Work &w)
-{
-    const mf_prefill_attention_args_t &a = p.a;
-    const int lane = threadIdx.x & 31;
+struct Ranking {
     Work seq[2];
-    int tiles[2], most = 0;
+    int tiles[2], most, all;
+    uint32_t inverse;  // 2^32 / tokens, rounded up
+
+    __device__ __forceinline__ void Begin(const Params &p)
+    {
+        const int lane = threadIdx.x & 31;
+        inverse = 0xffffffffu / (uint32_t)p.tokens + 1;
+        most = 0;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int b = lane * 2 + i;
-        seq[i].rows = seq[i].keys = 0;
-        if (b < a.B) {
-            Extent(a, b, seq[i]);
+        for (int i = 0; i < 2; i++) {
+            const int b = lane * 2 + i;
+            seq[i].rows = seq[i].keys = 0;
+            if (b < p.a.B) {
+                Extent(p.a, b, seq[i]);
+            }
+            tiles[i] = seq[i].rows > 0 ? Tiles(p, seq[i].rows - 1) + 1 : 0;
+            most = max(most, seq[i].keys > 0 ? (seq[i].keys - 1) / kTile + 1 : 0);
         }
-        tiles[i] = seq[i].rows > 0 ? (seq[i].rows + p.tokens - 1) / p.tokens : 0;
-        most = max(most, seq[i].keys > 0 ? (seq[i].keys + kTile - 1) / kTile : 0);
+        most = __reduce_max_sync(~0u, most);
+        all = Count(p, 0);
+    }
+    // n / tokens, 0 <= n: the product is too high by n / 2^32 < 1/2 at most before it is cut
+    __device__ __forceinline__ int Tiles(const Params &p, int n) const
+    {
+        const uint32_t t = __umulhi((uint32_t)n, inverse);
+        return (int)(t * (uint32_t)p.tokens > (uint32_t)n ? t - 1 : t);
     }
     // the first row tile of a sequence that takes m key tiles or more (its number of row tiles, if none does)
-    auto first = [&](int i, int m) {
-        const int need = (m - 1) * kTile + 1, past = seq[i].keys - seq[i].rows;
+    __device__ __forceinline__ int First(const Params &p, int i, int m) const
+    {
         if (m <= 0) {
             return 0;
         }
-        if (seq[i].keys < need) {
+        const int before = (m - 1) * kTile, past = seq[i].keys - seq[i].rows;
+        if (seq[i].keys <= before) {
             return tiles[i];
         }
-        return a.causal ? max(0, min(tiles[i] - 1, (need - past + p.tokens - 1) / p.tokens - 1)) : 0;
-    };
-    auto count = [&](int m) { return __reduce_add_sync(~0u, max(0, tiles[0] - first(0, m)) + max(0, tiles[1] - first(1, m))); };
-    int lo = 0, hi = __reduce_max_sync(~0u, most) + 1;  // count(lo) > number >= count(hi)
-    if (number >= count(0)) {
-        return false;
+        return p.a.causal ? max(0, min(tiles[i] - 1, Tiles(p, max(before - past, 0)))) : 0;
     }
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (count(mid) > number) {
-            lo = mid;
-        } else {
-            hi = mid;
+    __device__ __forceinline__ int Count(const Params &p, int m) const
+    {
+        return __reduce_add_sync(~0u, max(0, tiles[0] - First(p, 0, m)) + max(0, tiles[1] - First(p, 1, m)));
+    }
+    // Whole warp; false: an empty number.
+    __device__ __forceinline__ bool Find(const Params &p, int number, Work &w) const
+    {
+        const int lane = threadIdx.x & 31;
+        if (number >= all) {
+            return false;
         }
-    }
-    int at = number - count(lo + 1);  // among those that take `lo`
-    const int from[2] = {first(0, lo), first(1, lo)};
-    const int mine[2] = {max(0, first(0, lo + 1) - from[0]), max(0, first(1, lo + 1) - from[1])};
-    int before = mine[0] + mine[1];
+        int lo = 0, hi = most + 1;  // Count(lo) > number >= Count(hi)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (Count(p, mid) > number) {
+                lo = mid;
+            } else {
+                hi = mid;
+            }
+        }
+        const int from[2] = {First(p, 0, lo), First(p, 1, lo)};
+        const int to[2] = {First(p, 0, lo + 1), First(p, 1, lo + 1)};
+        int at = number - __reduce_add_sync(~0u, max(0, tiles[0] - to[0]) + max(0, tiles[1] - to[1]));  // among those that take `lo`
+        const int mine[2] = {max(0, to[0] - from[0]), max(0, to[1] - from[1])};
+        int before = mine[0] + mine[1];
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const int y = __shfl_up_sync(~0u, before, d);
-        before += lane >= d ? y : 0;
+        for (int d = 1; d < 32; d <<= 1) {
+            const int y = __shfl_up_sync(~0u, before, d);
+            before += lane >= d ? y : 0;
+        }
+        before -= mine[0] + mine[1];
+        const int which = at < before + mine[0] ? 0 : 1;
+        const unsigned owner = __ballot_sync(~0u, at >= before && at < before + mine[0] + mine[1]);
+        const int l = __ffs(owner) - 1;
+        at -= before + (which ? mine[0] : 0);
+        w.q0 = __shfl_sync(~0u, which ? seq[1].q0 : seq[0].q0, l);
+        w.rows = __shfl_sync(~0u, which ? seq[1].rows : seq[0].rows, l);
+        w.k0 = __shfl_sync(~0u, which ? seq[1].k0 : seq[0].k0, l);
+        w.keys = __shfl_sync(~0u, which ? seq[1].keys : seq[0].keys, l);
+        w.t0 = __shfl_sync(~0u, ((which ? from[1] : from[0]) + at) * p.tokens, l);
+        return owner != 0 && w.t0 < w.rows;
     }
-    before -= mine[0] + mine[1];
-    const int which = at < before + mine[0] ? 0 : 1;
-    const unsigned owner = __ballot_sync(~0u, at >= before && at < before + mine[0] + mine[1]);
-    const int l = __ffs(owner) - 1;
-    at -= before + (which ? mine[0] : 0);
-    w.q0 = __shfl_sync(~0u, which ? seq[1].q0 : seq[0].q0, l);
-    w.rows = __shfl_sync(~0u, which ? seq[1].rows : seq[0].rows, l);
-    w.k0 = __shfl_sync(~0u, which ? seq[1].k0 : seq[0].k0, l);
-    w.keys = __shfl_sync(~0u, which ? seq[1].keys : seq[0].keys, l);
-    w.t0 = __shfl_sync(~0u, ((which ? from[1] : from[0]) + at) * p.tokens, l);
-    return owner != 0 && w.t0 < w.rows;
-}
+};
 
 // A warp's view of the work list: the next two row tiles, or false at its end.
 template <int D>
@@ -350,13 +374,16 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
         if (warp == 10) {
             // ------------------------------------------------------------------ scheduler
             // Each unit of work is a CTA of the grid; a CTA that runs takes the next one that has not been launched yet when it begins with the one before.
-            int k = 0;
-            long long unit = blockIdx.x;
+            Ranking ranking;
+            if (a.B <= kRanked) {
+                ranking.Begin(p);
+            }
+            int k = 0, unit = (int)blockIdx.x;
             for (uint32_t claims = 0;; claims++) {
                 const bool end = unit < 0;
-                const int ht = (int)(unit % p.headTiles), number = (int)(unit / p.headTiles);
+                const int number = unit / p.headTiles, ht = unit - number * p.headTiles;
                 Work w = {0, 0, 0, 0, 0, -1, 0, 0};
-                const bool there = !end && (a.B <= kRanked ? Ranked(p, number, w) : Numbered(p, number, w));
+                const bool there = !end && (a.B <= kRanked ? ranking.Find(p, number, w) : Numbered(p, number, w));
                 if (there) {
                     const int see = a.causal ? min(w.keys, min(w.rows, w.t0 + p.tokens) + w.keys - w.rows) : w.keys;
                     w.n = see > 0 ? (see + kTile - 1) / kTile : 0;
@@ -646,6 +673,9 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
             const float2 both = Apart(Add2(part[0], part[1]));
             sum += both.x + both.y;
         };
+        // rows that the packing leaves over hold anything, and nobody looks at them
+        const int rowToken = i * half + row / p.pack, rowHead = row % p.pack;
+        const bool filled = row < p.pack * half;
         Worker<D> worker;
         Work w;
         uint32_t sPh = 0, oPh = 0;
@@ -654,9 +684,8 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
             if (i == 1 && w.t0 + half >= w.rows) {
                 continue;
             }
-            // rows that the packing leaves over hold anything, and nobody looks at them
-            const int token = row < p.pack * half ? w.t0 + i * half + row / p.pack : 0x7fffffff, past = w.keys - w.rows, head = w.h0 + row % p.pack;
-            const bool valid = token < w.rows;
+            const int token = w.t0 + rowToken, past = w.keys - w.rows, head = w.h0 + rowHead;
+            const bool valid = filled && token < w.rows;
             const int limit = a.causal && valid ? min(w.keys, token + past + 1) : w.keys;  // keys that the row sees
             const int sure = __reduce_min_sync(~0u, limit), most = __reduce_max_sync(~0u, valid ? limit : 0);
             top = -INFINITY;
