@@ -12,10 +12,18 @@ is contiguous (`block`): what `bm.copy_data_batch` moves between pools, if the d
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .attention import Plans, _misaligned, _ops, decode_attention, head_scales, int32, launch_on, no_gradient, on_gpu, one_word, strides, type_code
 from ..utils.tensors import current_stream_handle
+
+
+@functools.lru_cache(maxsize=64)
+def _plans(device, kind, kv_heads, head_dim):
+    """What the checks of writes and of requests have found, for all caches that they go by alike: a new one does not begin from nothing."""
+    return Plans(), Plans()
 
 
 class PagedKVCache:
@@ -46,7 +54,8 @@ class PagedKVCache:
         self.data, self.table, self.lengths, self.refs = data, table, lengths, refs
         self.status = status if status is not None else torch.zeros(1, dtype=torch.int32, device=data.device)
         self.seqs, self.width = table.shape
-        self._device, self._writes, self._requests = data.device, Plans(), Plans()
+        self._device = data.device
+        self._writes, self._requests = _plans(data.device, self._type, self.kv_heads, self.head_dim)
         self._native = _ops.KvCache(data.data_ptr(), table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), self.status.data_ptr(), self.layers, self.pages,
                                     self.page_size, self.kv_heads, self.head_dim * data.element_size(), self.seqs, self.width)
 

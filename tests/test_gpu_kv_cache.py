@@ -334,3 +334,65 @@ def test_cache_in_pooled_memory_whose_pages_are_moved_by_batch_copies(port):
     finally:
         torch.cuda.synchronize()
         pool.close()
+
+
+def test_caches_of_other_kinds_do_not_take_what_one_has_taken():
+    import torch
+
+    k = torch.ones(5, 2, 64, dtype=torch.bfloat16, device="cuda")
+    slots = torch.arange(5, device="cuda")
+    one, alike, fewer, longer, narrow = (_cache(1, 8, 4, *kind) for kind in
+                                         ((2, 64, 3, 4), (2, 64, 9, 2), (1, 64, 3, 4), (2, 128, 3, 4), (2, 64, 3, 4, "float8_e4m3fn")))
+    for cache in (one, alike):
+        for _ in range(2):
+            cache.write(0, k, k, slots)
+        assert torch.equal(cache.k_pages(0).transpose(1, 2).reshape(-1, 2, 64)[:5], k)
+    for cache in (fewer, longer, narrow):
+        with pytest.raises(ValueError):
+            cache.write(0, k, k, slots)
+    assert alike.reserve(_ints([8]), _ints([3]), 3).tolist() == [0, 1, 2] and alike.check_status() == 0
+    with pytest.raises(ValueError):
+        one.reserve(_ints([0, 1, 2, 0]), _ints([1, 1, 1, 1]), 4)
+    alike.reserve(_ints([0, 1, 2, 8]), _ints([1, 1, 1, 0]), 3)
+    assert alike.lengths.tolist() == [1, 1, 1, 0, 0, 0, 0, 0, 3] and alike.check_status() == 0
+
+
+FIRST_CALLS = """
+import torch
+from memfabric_hybrid_b200.ops.attention import prefill_attention, prefill_attention_reference
+from memfabric_hybrid_b200.ops.kv_cache import PagedKVCache
+
+ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+x = torch.randn(700, 12, 128, device="cuda", dtype=torch.bfloat16)
+q, k, v = x[:, :8], x[:, 8:10], x[:, 10:]
+cu, seqs, counts, third, one, rows = map(ints, ([0, 300, 700], [0, 1], [300, 400], [3], [1], [1, 1, 1]))
+cache = PagedKVCache.allocate(2, 64, 16, 2, 128, 6, 40)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    prompt = prefill_attention(q, k, v, cu)
+    cache.write(0, k, v, cache.reserve(seqs, counts, 700))
+    cache.fork(one, third)
+    cache.write(0, k[:1], v[:1], cache.reserve(third, one, 1))
+    step = cache.decode(0, q[:3], rows)
+    cache.free(one)
+    moved = cache.compact()
+graph.replay()
+torch.cuda.synchronize()
+assert cache.check_status() == 0 and cache.lengths.tolist() == [300, 0, 0, 401, 0, 0]
+assert int((cache.refs > 0).sum()) == 19 + 26 and bool((cache.refs[:45] == 1).all())
+want = prefill_attention_reference(q, k, v, cu)[0]
+assert float((prompt.double() - want).abs().max()) < 0.03
+keys, values = (t[300:].double().repeat_interleave(4, 1) for t in (k, v))
+weights = torch.softmax(torch.einsum("bhd,nhd->bhn", q[:3].double(), keys) * 128 ** -0.5, -1)
+assert float((step.double() - torch.einsum("bhn,nhd->bhd", weights, values)).abs().max()) < 0.03
+"""
+
+
+def test_a_process_may_begin_with_a_capture():
+    """Nothing that a first call sets up (attributes of kernels, plans) disturbs the capture of a graph."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
