@@ -218,7 +218,8 @@ __device__ __forceinline__ bool Numbered(const Params &p, int number, Work &w)
 
 // The same for a few sequences, with the row tiles in order of the key tiles that they take, the most first: what is left at the end is small. How many
 // row tiles take m key tiles or more follows from a sequence's lengths; the m of a number is found by bisection. A lane has two sequences, the lengths of
-// which stay in registers, and divides by multiplying.
+// which stay in registers, and divides by multiplying: with lengths loaded and divided for each number a search took 7000 cycles instead of 2300, and short
+// prompts, whose row tiles take 8000, waited for it (31 of up to 190 tokens 27.6 against 24.8 us).
 constexpr int kRanked = 64;
 struct Ranking {
     Work seq[2];
