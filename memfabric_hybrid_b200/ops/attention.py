@@ -26,7 +26,7 @@ def type_code(dtype):
     """The kernels' number of an element type, None for one that they do not know."""
     global _types
     if _types is None:
-            _types = {torch.bfloat16: _ops.BF16, torch.float16: _ops.FP16, torch.float8_e4m3fn: _ops.E4M3}
+        _types = {torch.bfloat16: _ops.BF16, torch.float16: _ops.FP16, torch.float8_e4m3fn: _ops.E4M3}
     return _types.get(dtype)
 
 
@@ -59,8 +59,11 @@ _here = contextlib.nullcontext()
 
 def launch_on(device, stream):
     """A context in which what is allocated belongs to the stream that will use it, on GPU number `device`."""
-    if stream is None and torch._C._cuda_getDevice() == device:
-        return _here
+    if stream is None:
+        if torch._C._cuda_getDevice() == device:
+            return _here
+    elif stream.device.index != device:
+        raise ValueError(f"the stream belongs to {stream.device}, the tensors are on cuda:{device}")
     return _elsewhere(device, stream)
 
 

@@ -89,3 +89,12 @@ def test_cache_refuses(kw):
          "refs": torch.zeros(5, dtype=torch.int32)} | kw
     with pytest.raises(ValueError):
         PagedKVCache(**a)
+
+
+def test_a_stream_of_another_gpu_is_refused():
+    from types import SimpleNamespace
+
+    from memfabric_hybrid_b200.ops.attention import launch_on
+
+    with pytest.raises(ValueError, match="the stream belongs to cuda:1"):
+        launch_on(0, SimpleNamespace(device=torch.device("cuda", 1)))
