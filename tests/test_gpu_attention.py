@@ -485,6 +485,29 @@ def test_offsets_that_leave_the_tensors_are_cut_off():
     assert bool((room[:20] == 5).all() and (room[120:] == 5).all())
 
 
+@pytest.mark.parametrize("batch", [3, 64, 65, 700])
+def test_offsets_of_any_content_stay_inside(batch):
+    """Offsets in no order, out of range and at the ends of their type: nothing outside is written. (What lies inside is not defined then.)"""
+    import torch
+
+    from memfabric_hybrid_b200.ops import attention as A
+
+    g = torch.Generator().manual_seed(batch)
+    for heads, kv_heads in ((4, 2), (6, 2), (7, 7)):
+        q, k, v = _q((300, heads, 64), torch.bfloat16, 1), _q((290, kv_heads, 64), torch.bfloat16, 2), _q((290, kv_heads, 64), torch.bfloat16, 3)
+        room, lse = torch.full((340, heads, 64), 5.0, dtype=torch.bfloat16, device="cuda"), torch.full((340, heads), 5.0, device="cuda")
+        for _ in range(4):
+            cu = []
+            for _ in range(2):
+                x = torch.randint(-50, 400, (batch + 1,), generator=g)
+                odd = torch.randint(0, 6, (batch + 1,), generator=g)
+                x = torch.where(odd == 0, -2 ** 31, torch.where(odd == 1, 2 ** 31 - 1, x))
+                cu.append(x.to(torch.int32).cuda())
+            A.prefill_attention(q, k, v, *cu, out=room[20:320], lse=lse[20:320])
+            torch.cuda.synchronize()
+        assert bool((room[:20] == 5).all() and (room[320:] == 5).all() and (lse[:20] == 5).all() and (lse[320:] == 5).all())
+
+
 def test_prefill_offsets_past_32_bits():
     """Queries, keys, values and results of more than 2^32 bytes each: the last prompts of many against the same ones alone."""
     import torch
