@@ -476,9 +476,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode
                         LdMatrix4T(m, vAt + X::Place(block * 16 + (lane & 15), s + (lane >> 4)));
 #pragma unroll
                         for (int c = 0; c < 2; c++) {
-                            const uint32_t lo = m[2 * c], hi = m[2 * c + 1];
-                            const uint32_t a0 = E4m3ToHalf2(__byte_perm(lo, 0, 0x4420)), a1 = E4m3ToHalf2(__byte_perm(lo, 0, 0x4431)),
-                                           a2 = E4m3ToHalf2(__byte_perm(hi, 0, 0x4420)), a3 = E4m3ToHalf2(__byte_perm(hi, 0, 0x4431));
+                            const uint32_t lo = __byte_perm(m[2 * c], 0, 0x3120), hi = __byte_perm(m[2 * c + 1], 0, 0x3120);
+                            const uint32_t a0 = E4m3ToHalf2(lo), a1 = E4m3ToHalf2(lo >> 16), a2 = E4m3ToHalf2(hi), a3 = E4m3ToHalf2(hi >> 16);
 #pragma unroll
                             for (int t = 0; t < NT; t++) {
                                 Mma16x8x16<T>(acc[t][s + c], a0, a1, a2, a3, p[t][0], p[t][1]);
