@@ -47,6 +47,14 @@ __device__ __forceinline__ void LdMatrix4T(uint32_t (&r)[4], uint32_t addr)
                  : "r"(addr)
                  : "memory");
 }
+// Two matrices of 16 rows of 16 bytes, transposed: r[0], r[1] hold columns lane / 4 and lane / 4 + 8 of the first, rows 4 (lane % 4) and the next three.
+__device__ __forceinline__ void LdMatrix2T8(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
 
 // The 8 x 8 matrix of 16-bit values that a warp holds (row lane / 4, columns 2 (lane % 4) and the next), transposed.
 __device__ __forceinline__ uint32_t Transposed8x8(uint32_t v)

@@ -61,9 +61,16 @@ struct Cfg {
     static constexpr uint32_t kSmem = kWarps * kRing + kJoins * kRows * kJoinRow * 4;
     static __device__ __forceinline__ uint32_t Place(uint32_t row, uint32_t chunk)
     {
-        const uint32_t x = kRow >= 128 ? row & 7 : (row >> 1) & 3;  // eight rows of one chunk lie in eight different bank groups
+        // eight rows of one chunk lie in eight different bank groups: rows 0-7, 8-15, and of 8-bit ones also Key(0) to Key(7), Key(8) to Key(15)
+        uint32_t x = kRow >= 128 ? row & 7 : (row >> 1) & 3;
+        if (sizeof(C) == 1) {
+            x ^= row >> 3 & 1 ? (kRow >= 128 ? 2 : 1) : 0;
+        }
         return row * kRow + ((chunk ^ x) << 4);
     }
+    // The key of a block that is row `row` of its products. The transposing load of 8-bit values gives a lane four neighbouring keys, which the second
+    // product takes as two pairs, eight rows apart.
+    static __device__ __forceinline__ int Key(int row) { return sizeof(C) == 1 ? (row & 6) * 2 + (row & 1) + (row >> 3) * 2 : row; }
 };
 
 // The row that a position of the line of tiles lies in.
@@ -374,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode
         if (key0 < cur.length) {
             // A block behind the end of the sequence holds what was there before: its scores are masked, its values left alone.
             const int blocks = kBlocks == 1 ? 1 : min(kBlocks, (cur.length - key0 + 15) / 16);
-            float x[kBlocks][NT][4];  // [key quad, quad + 8][head 2 pos, 2 pos + 1]
+            float x[kBlocks][NT][4];  // [row quad, quad + 8][head 2 pos, 2 pos + 1]
             bool grown = false;
 #pragma unroll
             for (int block = 0; block < kBlocks; block++) {
@@ -387,11 +394,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode
                     }
                 }
                 if (kWide) {
-                    // matrices: keys 0-7 and 8-15 of one chunk, the same of the next; four neighbouring columns to a lane
+                    // matrices: rows 0-7 and 8-15 of one chunk, the same of the next; four neighbouring columns to a lane
 #pragma unroll
                     for (int s = 0; s < kSteps; s += 2) {
                         uint32_t m[4];
-                        LdMatrix4(m, at + X::Place(block * 16 + (lane & 15), s + (lane >> 4)));
+                        LdMatrix4(m, at + X::Place(block * 16 + X::Key(lane & 15), s + (lane >> 4)));
 #pragma unroll
                         for (int c = 0; c < 2; c++) {
                             const uint32_t a0 = E4m3ToHalf2(m[2 * c]), a1 = E4m3ToHalf2(m[2 * c + 1]), a2 = E4m3ToHalf2(m[2 * c] >> 16),
@@ -418,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode
                 for (int t = 0; t < NT; t++) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const bool seen = key0 + block * 16 + quad + (e >> 1) * 8 < cur.length;
+                        const bool seen = key0 + block * 16 + X::Key(quad + (e >> 1) * 8) < cur.length;
                         x[block][t][e] = seen ? (y[0][t][e] + y[1][t][e]) * factor[t][e & 1] : -INFINITY;
                         grown |= x[block][t][e] - top[t][e & 1] > Weights<T>::kSlack;
                     }
@@ -468,16 +475,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode
                     p[t][1] = Transposed8x8(Pack2<T>(x[block][t][2], x[block][t][3]));
                 }
                 if (kWide) {
-                    // matrices, transposed: keys 0-7 and 8-15 of a chunk, the same of the next. A 16-bit unit holds an even and an odd column of one key:
-                    // even columns are the first eight rows of the product, odd ones the others.
+                    // matrices of 16 keys and 16 columns, transposed: two chunks, of each columns 0-7 and 8-15; four neighbouring keys to a lane
 #pragma unroll
                     for (int s = 0; s < kSteps; s += 2) {
                         uint32_t m[4];
-                        LdMatrix4T(m, vAt + X::Place(block * 16 + (lane & 15), s + (lane >> 4)));
+                        LdMatrix2T8(m, vAt + X::Place(block * 16 + (lane & 15), s + (lane >> 4)));
 #pragma unroll
                         for (int c = 0; c < 2; c++) {
-                            const uint32_t lo = __byte_perm(m[2 * c], 0, 0x3120), hi = __byte_perm(m[2 * c + 1], 0, 0x3120);
-                            const uint32_t a0 = E4m3ToHalf2(lo), a1 = E4m3ToHalf2(lo >> 16), a2 = E4m3ToHalf2(hi), a3 = E4m3ToHalf2(hi >> 16);
+                            const uint32_t a0 = E4m3ToHalf2(m[2 * c]), a1 = E4m3ToHalf2(m[2 * c + 1]), a2 = E4m3ToHalf2(m[2 * c] >> 16),
+                                           a3 = E4m3ToHalf2(m[2 * c + 1] >> 16);
 #pragma unroll
                             for (int t = 0; t < NT; t++) {
                                 Mma16x8x16<T>(acc[t][s + c], a0, a1, a2, a3, p[t][0], p[t][1]);
@@ -544,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode
                         for (int t = 0; t < NT; t++) {
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
-                                const int d = s * 16 + (kWide ? 2 * quad + (e >> 1) : quad + (e >> 1) * 8);
+                                const int d = s * 16 + quad + (e >> 1) * 8;
                                 float *place = mine + (t * 8 + 2 * pos + (e & 1)) * X::kJoinRow + d;
                                 const float y = acc[t][s][e] * weight[t][e & 1];
                                 *place = turn == 0 ? y : *place + y;
