@@ -260,6 +260,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode
     const uint32_t ring = SmemAddr32(smem) + warp * X::kRing;
     float *join = (float *)(smem + kWarps * X::kRing);
     const bool together = a.pageSize % 16 == 0;  // 16 keys from a multiple of 16 on lie in one page
+    constexpr int kPer = 32 / X::kChunks;        // rows that the warp copies in one trip
+    const long long perKey = a.stride[2] * (long long)sizeof(C), perTrip = kPer * perKey, kToV = (const unsigned char *)a.v - (const unsigned char *)a.k,
+                    lanePart = lane / X::kChunks * perKey + lane % X::kChunks * 16;
     Cursor ahead = cur;
     long long aheadLeft = left;
     uint32_t fill = 0;
@@ -286,7 +289,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode
                     }
                 }
                 const uint32_t at = ring + fill * X::kStage;
-                constexpr int kPer = 32 / X::kChunks;  // rows of one trip
+                if (together && own >= 0 && key0 + 16 <= ahead.length) {  // all sixteen, a fixed number of bytes apart
+                    const unsigned char *from = (const unsigned char *)a.k + own * (long long)sizeof(C) + lanePart;
+#pragma unroll
+                    for (int i = 0; i < 16 / kPer; i++) {
+                        const uint32_t to = at + X::Place(block * 16 + i * kPer + lane / X::kChunks, lane % X::kChunks);
+                        CpAsync16(to, from, 16);
+                        CpAsync16(to + kWarpKeys * X::kRow, from + kToV, 16);
+                        from += perTrip;
+                    }
+                    continue;
+                }
 #pragma unroll
                 for (int i = 0; i < 16 / kPer; i++) {
                     const uint32_t row = i * kPer + lane / X::kChunks, chunk = lane % X::kChunks;
