@@ -6,11 +6,11 @@
 // value is read once and takes part in 4 * group operations per element, so what counts is that all SMs stream, all the time, whatever
 // the lengths are.
 //
-// Work split. The keys of every (sequence, cache head) are cut into tiles of 64; the tiles of all rows form one line, and each CTA takes an
+// Work split. The keys of every (sequence, cache head) are cut into tiles of 64 to 256; the tiles of all rows form one line, and each CTA takes an
 // equal, contiguous piece of it, whichever rows that touches (lengths live on the device: the host sizes the grid only). A row that lies
 // within one CTA is written at once; of a row that crosses CTAs each leaves maximum, sum and unnormalised output in the workspace,
-// at most two per CTA, and a second kernel joins them in the order of the CTAs, so results do not depend on timing. Where no row has more
-// than kWholeKeys keys, CTAs take whole rows and nothing has to be joined.
+// at most two per CTA, and a second kernel joins them in the order of the CTAs, so results do not depend on timing. Where all rows are
+// short (kWholeTiles), CTAs take whole rows and nothing has to be joined.
 //
 // A CTA is four warps that share nothing but their position: each takes a quarter of the keys of every tile, fetches them through its own ring
 // of cp.async stages (rows past the end of the sequence are filled with zeros: stale pages may hold anything, NaN included) and keeps its
@@ -36,8 +36,7 @@ using mf::sm100::GridDependency;
 constexpr int kThreads = 128;
 constexpr int kMostCtasPerSm = 3;
 constexpr int kWarps = 4;
-constexpr int kWholeKeys = 256;
-constexpr int kRowCost = 2;        // tiles that beginning and ending a row takes as long as (0: 61 ragged sequences 83 us, 1 to 3: 79)
+constexpr int kWholeKeys = 256;    // rows up to here are never cut: no workspace
 constexpr int kPartialFloats = 2;  // maximum and sum before a row's values
 constexpr int kLeastPiece = 2;
 constexpr int kJoinGroups = 4;     // of threads that share the parts of a row in the second kernel
@@ -46,12 +45,19 @@ template <typename C, int D, int NT>
 struct Cfg {
     static constexpr uint32_t kRow = D * sizeof(C);
     static constexpr uint32_t kChunks = kRow / 16;
-    // Blocks of 16 keys that a warp works on in one step: as many as make 8 KiB of keys and values (D = 64, e4m3, 200 sequences: two 142, four 117 us).
+    // Blocks of 16 keys that a warp works on in one step: as many as make 8 KiB of keys and values (D = 64, e4m3, 200 sequences: two 109, four 102 us).
     static constexpr int kBlocks = 256 / kRow;
-    static constexpr int kWarpKeys = 16 * kBlocks, kTileKeys = kWarps * kWarpKeys, kWholeTiles = kWholeKeys / kTileKeys;
+    static constexpr int kWarpKeys = 16 * kBlocks, kTileKeys = kWarps * kWarpKeys;
+    // Where all rows are this short none is cut. Two tiles of 256 keys (e4m3 of 64 values): 8 sequences of 500 tokens 12.0 -> 10.3 us, 200 of 1024 the same;
+    // four tiles everywhere: 200 of up to 512 tokens 33 -> 39.
+    static constexpr int kWholeTiles = kWholeKeys / kTileKeys > 2 ? kWholeKeys / kTileKeys : 2;
+    static_assert(kWholeTiles * kTileKeys >= kWholeKeys, "rows without a workspace are not cut");
+    // Tiles that beginning and ending a row takes as long as; its queries and results grow with D. 0 / 1 / 2 / 3 tiles: D = 128, 61 ragged sequences 79.5,
+    // 77.4, 76.9, 77.8 us, 200 of up to 1200 tokens 90.9, 76.5, 73.2, 73.4; D = 64, e4m3, 200 ragged ones 114, 102, 115, 133.
+    static constexpr int kRowCost = D / 64;
     static constexpr uint32_t kStage = kWarpKeys * kRow * 2;  // keys and values of a warp's part of a tile
-    // Where a block of keys takes many instructions for its bytes (8-bit ones), three CTAs per SM with two stages hide more than two with three: 135 ->
-    // 127 us for 128 sequences of e4m3; with 16-bit rows of 64 values 68 -> 79 us.
+    // Where a block of keys takes many instructions for its bytes (8-bit ones), three CTAs per SM with two stages hide more than two with three: 116 ->
+    // 113 us for 128 sequences of e4m3, of 64 values 121 -> 115; with 16-bit rows of 64 values 95 -> 116 us.
     static constexpr int kCtasPerSm = sizeof(C) == 1 && NT == 1 ? 3 : 2;
     static constexpr int kStages = (kCtasPerSm == 3 ? 16384 : 24576) / kStage;
     static constexpr uint32_t kRing = kStages * kStage;
@@ -159,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode
     int longest = 0;
     for (int b = b0; b < b1; b++) {
         const int n = L::Tiles(line.Length(b));
-        tiles += n > 0 ? n + kRowCost : 0;
+        tiles += n > 0 ? n + X::kRowCost : 0;
         rows += n > 0;
         longest = max(longest, n);
     }
@@ -194,9 +200,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode
         longest = max(longest, scanMax[w]);
     }
     const bool whole = longest <= X::kWholeTiles;
-    // The line in units: a row is kRowCost of them, then one for each tile; or one if rows are not cut. A piece is worth a CTA from
+    // The line in units: a row is X::kRowCost of them, then one for each tile; or one if rows are not cut. A piece is worth a CTA from
     // kLeastPiece units on; the CTAs behind the last piece have none.
-    const int price = whole ? 1 : kRowCost;
+    const int price = whole ? 1 : X::kRowCost;
     const long long units = (whole ? total[1] : total[0]) * HG, wanted = whole ? units : (units + kLeastPiece - 1) / kLeastPiece,
                     parts = wanted < gridDim.x ? wanted : gridDim.x;
     long long first = 0, last = 0;
