@@ -39,7 +39,9 @@ constexpr int kWarps = 4;
 constexpr int kWholeKeys = 256;    // rows up to here are never cut: no workspace
 constexpr int kPartialFloats = 2;  // maximum and sum before a row's values
 constexpr int kLeastPiece = 2;
-constexpr int kJoinGroups = 4;     // of threads that share the parts of a row in the second kernel
+// Groups of threads that share the parts of a row in the second kernel. 61 sequences: two 77.9, four 77.1 us; with 16 query heads per key head 82.6 and 84.3.
+template <int NT>
+constexpr int kJoinGroups = 4 / NT;
 
 template <typename C, int D, int NT>
 struct Cfg {
@@ -630,48 +632,62 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode
 // One CTA for each row that is continued behind CTA blockIdx.x of the first kernel: that one's second partial result and the first ones
 // of the CTAs behind it, as long as they are of the same row. A thread owns eight columns of a query head.
 template <typename Q, int D, bool WIDE, int NT>
-__global__ void __launch_bounds__(NT * D * kJoinGroups) mf_decode_join_kernel(const __grid_constant__ mf_decode_attention_args_t a, int ctas)
+__global__ void __launch_bounds__(NT * D * kJoinGroups<NT>) mf_decode_join_kernel(const __grid_constant__ mf_decode_attention_args_t a, int ctas)
 {
     constexpr int kRows = 8 * NT;
     GridDependency();
     const int2 *marks = (const int2 *)a.marks;
     const int c = blockIdx.x;
+    const int group = threadIdx.x / (NT * D), r = threadIdx.x % (NT * D) / (D / 8), d = (threadIdx.x % (D / 8)) * 8;
+    // The first mark of each thread and the first part of each group are fetched before it is known how many there are (500 tokens each of 8 sequences 11.8 ->
+    // 10.8 us); whatever stands there otherwise is left alone.
     const int2 row = marks[2 * c + 1];
+    const int near = c + 1 + (int)threadIdx.x;
+    const int2 mark0 = near < ctas ? marks[2 * near] : make_int2(-1, -1);
+    const float *ws0 = Partial<D, kRows>((float *)a.workspace, min(c + group, ctas - 1), group == 0 ? 1 : 0);
+    const float2 ms0 = *(const float2 *)(ws0 + r * kPartialFloats);
+    const float4 x0 = *(const float4 *)(ws0 + kRows * kPartialFloats + r * D + d), y0 = *(const float4 *)(ws0 + kRows * kPartialFloats + r * D + d + 4);
     if (row.x < 0) {
         return;
     }
     const int GT = (a.group + kRows - 1) / kRows, kvh = row.y / GT, g = (row.y % GT) * kRows;
-    const int group = threadIdx.x / (NT * D), r = threadIdx.x % (NT * D) / (D / 8), d = (threadIdx.x % (D / 8)) * 8;
     // the CTAs behind that hold a part of the row: all marks at once
     __shared__ int behind;
     if (threadIdx.x == 0) {
         behind = ctas;
     }
     __syncthreads();
-    for (int i = c + 1 + threadIdx.x; i < ctas; i += blockDim.x) {
-        const int2 m = marks[2 * i];
+    for (int i = near; i < ctas; i += blockDim.x) {
+        const int2 m = i == near ? mark0 : marks[2 * i];
         if (m.x != row.x || m.y != row.y) {
             atomicMin(&behind, i);
         }
     }
     __syncthreads();
     const int n = behind - c;
-    float best = -INFINITY, all = 0, out[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    const bool any = group < n;
+    float best = any ? ms0.x : -INFINITY, all = any ? ms0.y : 0;
+    float out[8] = {x0.x, x0.y, x0.z, x0.w, y0.x, y0.y, y0.z, y0.w};
+    if (!any) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            out[j] = 0;
+        }
+    }
     constexpr int kAhead = 4;  // parts whose loads are in flight together
-    const int from = n * group / kJoinGroups, to = n * (group + 1) / kJoinGroups;  // in order: a group's parts lie before the next one's
-    for (int i = from; i < to; i += kAhead) {
+    for (int i = group + kJoinGroups<NT>; i < n; i += kAhead * kJoinGroups<NT>) {
         float2 ms[kAhead];
         float4 x[kAhead], y[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; u++) {
-            const float *ws = Partial<D, kRows>((float *)a.workspace, c + min(i + u, to - 1), min(i + u, to - 1) == 0 ? 1 : 0);
+            const float *ws = Partial<D, kRows>((float *)a.workspace, c + min(i + u * kJoinGroups<NT>, n - 1), 0);
             ms[u] = *(const float2 *)(ws + r * kPartialFloats);
             x[u] = *(const float4 *)(ws + kRows * kPartialFloats + r * D + d);
             y[u] = *(const float4 *)(ws + kRows * kPartialFloats + r * D + d + 4);
         }
 #pragma unroll
         for (int u = 0; u < kAhead; u++) {
-            if (i + u < to) {
+            if (i + u * kJoinGroups<NT> < n) {
                 const float next = fmaxf(best, ms[u].x), base = next == -INFINITY ? 0.0f : next;
                 const float keep = Exp2(best - base), weight = Exp2(ms[u].x - base);
                 const float v[8] = {x[u].x, x[u].y, x[u].z, x[u].w, y[u].x, y[u].y, y[u].z, y[u].w};
@@ -684,8 +700,8 @@ __global__ void __launch_bounds__(NT * D * kJoinGroups) mf_decode_join_kernel(co
             }
         }
     }
-    __shared__ float tops[kJoinGroups][kRows], sums[kJoinGroups][kRows];
-    __shared__ __align__(16) float values[kJoinGroups][kRows * D];
+    __shared__ float tops[kJoinGroups<NT>][kRows], sums[kJoinGroups<NT>][kRows];
+    __shared__ __align__(16) float values[kJoinGroups<NT>][kRows * D];
     if (d == 0) {
         tops[group][r] = best;
         sums[group][r] = all;
@@ -697,7 +713,7 @@ __global__ void __launch_bounds__(NT * D * kJoinGroups) mf_decode_join_kernel(co
         return;
     }
 #pragma unroll
-    for (int i = 1; i < kJoinGroups; i++) {
+    for (int i = 1; i < kJoinGroups<NT>; i++) {
         const float next = fmaxf(best, tops[i][r]), base = next == -INFINITY ? 0.0f : next;
         const float keep = Exp2(best - base), weight = Exp2(tops[i][r] - base);
         best = next;
@@ -747,7 +763,7 @@ int Launch(const mf_decode_attention_args_t &a, int ctas, cudaStream_t stream)
     }
     // rows of at most kWholeKeys keys are never cut
     if ((long long)a.tableWidth * a.pageSize > kWholeKeys &&
-        mf::sm100::LaunchDependent(mf_decode_join_kernel<Q, D, sizeof(C) == 1, NT>, ctas, NT * D * kJoinGroups, 0, stream, a, ctas) != cudaSuccess) {
+        mf::sm100::LaunchDependent(mf_decode_join_kernel<Q, D, sizeof(C) == 1, NT>, ctas, NT * D * kJoinGroups<NT>, 0, stream, a, ctas) != cudaSuccess) {
         (void)cudaGetLastError();
         return MF_K_LAUNCH_FAILED;
     }
