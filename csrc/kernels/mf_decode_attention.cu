@@ -284,21 +284,21 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode
                 if (key0 >= ahead.length) {
                     break;
                 }
-                // each lane looks the first or one of the 16 rows up: its offset in elements, or -1
+                // each lane looks the first or one of the 16 rows up: its offset in bytes, or -1
                 const int key = key0 + (together ? 0 : lane & 15);
                 long long own = -1;
                 if (key < ahead.length) {
                     const uint32_t page = a.pageSize == 1 ? key : __umulhi((uint32_t)key, a.pageMagic) >> a.pageShift;
                     const int p = entry[page];
                     if (p >= 0 && p < a.pages) {
-                        own = p * a.stride[0] + head + (long long)((uint32_t)key - page * (uint32_t)a.pageSize) * a.stride[2];
+                        own = (p * a.stride[0] + head) * (long long)sizeof(C) + (long long)((uint32_t)key - page * (uint32_t)a.pageSize) * perKey;
                     } else if (a.status != nullptr) {
                         *a.status = MF_DEV_ERR_BOUNDS;
                     }
                 }
                 const uint32_t at = ring + fill * X::kStage;
                 if (together && own >= 0 && key0 + 16 <= ahead.length) {  // all sixteen, a fixed number of bytes apart
-                    const unsigned char *from = (const unsigned char *)a.k + own * (long long)sizeof(C) + lanePart;
+                    const unsigned char *from = (const unsigned char *)a.k + own + lanePart;
 #pragma unroll
                     for (int i = 0; i < 16 / kPer; i++) {
                         const uint32_t to = at + X::Place(block * 16 + i * kPer + lane / X::kChunks, lane % X::kChunks);
@@ -311,12 +311,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode
 #pragma unroll
                 for (int i = 0; i < 16 / kPer; i++) {
                     const uint32_t row = i * kPer + lane / X::kChunks, chunk = lane % X::kChunks;
-                    const long long o = together ? own : __shfl_sync(~0u, own, row);
-                    const bool there = o >= 0 && key0 + (int)row < ahead.length;
-                    const size_t from = there ? (size_t)(o + (together ? row * a.stride[2] : 0)) * sizeof(C) + chunk * 16 : 0;
+                    const long long o = together ? own + row * perKey : __shfl_sync(~0u, own, row);
+                    const bool there = together ? own >= 0 && key0 + (int)row < ahead.length : o >= 0;
+                    const unsigned char *from = (const unsigned char *)a.k + (there ? o + chunk * 16 : 0);
                     const uint32_t to = at + X::Place(block * 16 + row, chunk);
-                    CpAsync16(to, (const unsigned char *)a.k + from, there ? 16 : 0);
-                    CpAsync16(to + kWarpKeys * X::kRow, (const unsigned char *)a.v + from, there ? 16 : 0);
+                    CpAsync16(to, from, there ? 16 : 0);
+                    CpAsync16(to + kWarpKeys * X::kRow, from + kToV, there ? 16 : 0);
                 }
             }
             next(ahead, aheadLeft);
