@@ -116,6 +116,30 @@ def test_decode_page_sizes(page, dim):
     _decode_case([0, 1, page, page + 1, 3 * page - 1, 400], page, 4, 2, dim, torch.float16)
 
 
+@pytest.mark.parametrize("lengths", [[256, 255, 1], [257, 256, 3], [511, 512, 0, 12], [513, 512], [512] * 40, [1024, 700, 1025], [640] * 9])
+@pytest.mark.parametrize("page", [16, 64, 9])
+@pytest.mark.parametrize("dim,cache", [(64, None), (64, "float8_e4m3fn"), (128, "float8_e4m3fn")])
+def test_decode_at_the_lengths_from_which_rows_are_cut(lengths, page, dim, cache):
+    import torch
+
+    _decode_case(lengths, page, 8, 2, dim, torch.bfloat16, cache=getattr(torch, cache) if cache else None)
+
+
+def test_decode_values_that_lie_before_the_keys():
+    import torch
+
+    from memfabric_hybrid_b200.ops import attention as A
+
+    for dtype in (torch.float16, torch.float8_e4m3fn):
+        k, v, table, lens = _pool([300, 77, 1200], 16, 2, 64, dtype)
+        scales = {"k_scale": torch.full((2,), 0.01, device="cuda"), "v_scale": torch.full((2,), 0.02, device="cuda")} if dtype == torch.float8_e4m3fn else {}
+        q = _q((3, 8, 64), torch.float16)
+        want = A.decode_attention(q, k.view(torch.uint8).contiguous().view(dtype), v.view(torch.uint8).contiguous().view(dtype), table, lens, **scales)
+        turned = torch.stack((v.view(torch.uint8), k.view(torch.uint8)), 1).view(dtype)
+        assert turned[:, 0].data_ptr() < turned[:, 1].data_ptr()
+        assert torch.equal(A.decode_attention(q, turned[:, 1], turned[:, 0], table, lens, **scales), want)
+
+
 def test_decode_rows_in_any_order_and_twice():
     import torch
 
