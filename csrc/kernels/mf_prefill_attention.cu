@@ -72,10 +72,17 @@ struct Params {
     int tiles;     // numbers of row tiles, empty ones among them
 };
 
-__device__ __forceinline__ float Max3(float a, float b, float c)
+// The largest; NaN if there is one among them.
+__device__ __forceinline__ float MaxNan(float a, float b)
 {
     float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float MaxNan(float a, float b, float c)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 __device__ __forceinline__ uint64_t Both(float lo, float hi)
@@ -108,36 +115,29 @@ __device__ __forceinline__ uint64_t Mul2(uint64_t a, uint64_t b)
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-__device__ __forceinline__ float AtLeast(float x, float least)
-{
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(least));
-    return r;
-}
-
 // 2^x for x <= 16 on the FMA pipe, for a share of the weights: the special function unit gives 16 results a cycle and SM, which is as long for a tile
 // as its MMAs take at D = 128. x = n + f with n the nearest whole number (W. J. Cody, W. Waite, "Software Manual for the Elementary
-// Functions", 1980), 2^f by the polynomial of least relative error on [-1/2, 1/2] (Remez exchange; 7.5e-5 of degree 3, 2.7e-6 of degree 4,
-// below the rounding of p to bf16 and fp16), n added to its exponent. Below -126 the result stays near 2^-126 (the exponent field must not fall below 0); NaN comes out as an
-// infinite or huge p, which has the row computed again.
+// Functions", 1980), 2^f by the polynomial of least relative error on [-1/2, 1/2] among those that are 1 at 0 (linear program; 1.01e-4 of degree 3, 2.9e-6
+// of degree 4, below the rounding of p to bf16 and fp16), n added to its exponent. That 1 makes masked weights exactly 0: whatever lies below -127 is
+// taken for -127, where the bits of 1 less 127 exponents are none. With a least weight above 0, v of a masked key reaches the row if it is large enough.
+// Between -127 and -126 the result lies below 2^-126. NaN comes out as 0: the row's sum knows about it.
 template <bool BF16>
 __device__ __forceinline__ float2 Exp2Poly(uint64_t x2)
 {
     const float2 x = Apart(x2);
-    x2 = Both(AtLeast(x.x, -126.0f), AtLeast(x.y, -126.0f));
+    x2 = Both(fmaxf(x.x, -127.0f), fmaxf(x.y, -127.0f));
     const uint64_t r2 = Add2(x2, Both(12582912.0f, 12582912.0f));  // 1.5 * 2^23: n stands in the lowest bits
     const uint64_t f2 = Fma2(Add2(r2, Both(-12582912.0f, -12582912.0f)), Both(-1.0f, -1.0f), x2);
     uint64_t p2;
     if (BF16) {
-        p2 = Fma2(Both(0.055171669f, 0.055171669f), f2, Both(0.242611122f, 0.242611122f));
-        p2 = Fma2(p2, f2, Both(0.693260985f, 0.693260985f));
-        p2 = Fma2(p2, f2, Both(0.999928074f, 0.999928074f));
+        p2 = Fma2(Both(0.055008932f, 0.055008932f), f2, Both(0.242210959f, 0.242210959f));
+        p2 = Fma2(p2, f2, Both(0.693282927f, 0.693282927f));
     } else {
-        p2 = Fma2(Both(0.009570102f, 0.009570102f), f2, Both(0.055917860f, 0.055917860f));
-        p2 = Fma2(p2, f2, Both(0.240247448f, 0.240247448f));
-        p2 = Fma2(p2, f2, Both(0.693121815f, 0.693121815f));
-        p2 = Fma2(p2, f2, Both(0.999999261f, 0.999999261f));
+        p2 = Fma2(Both(0.009582853f, 0.009582853f), f2, Both(0.055906425f, 0.055906425f));
+        p2 = Fma2(p2, f2, Both(0.240240986f, 0.240240986f));
+        p2 = Fma2(p2, f2, Both(0.693124193f, 0.693124193f));
     }
+    p2 = Fma2(p2, f2, Both(1.0f, 1.0f));
     const float2 r = Apart(r2), p = Apart(p2);
     return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(r.x) << 23)), __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23)));
 }
@@ -608,14 +608,15 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
             for (int c = 4; c < kTile - 4; c += 8) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    m[e] = Max3(m[e], x[c + e], x[c + 4 + e]);
+                    m[e] = MaxNan(m[e], x[c + e], x[c + 4 + e]);
                 }
             }
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                m[e] = fmaxf(m[e], x[kTile - 4 + e]);
+                m[e] = MaxNan(m[e], x[kTile - 4 + e]);
             }
-            const float best = Max3(fmaxf(m[0], m[1]), m[2], m[3]);
+            const float best = MaxNan(MaxNan(m[0], m[1]), m[2], m[3]);
+            sum = best < INFINITY ? sum : NAN;  // a logit that is NaN or infinite: so is the row, whatever its weights come out as
             const bool grown = (best - top) * factor > Weights<T>::kSlack;
             if (__any_sync(~0u, grown)) {
                 const float shrink = grown ? Exp2((top - best + lift) * factor) : 1.0f;
@@ -709,8 +710,8 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
             }
             oPh ^= w.n > 0 ? 1 : 0;
             TcFenceAfter();
-            // ---- O / sum. A row that saw no key has weights of 2^-126 from Exp2Poly: it is known by its reference.
-            const float scale = top != -INFINITY || sum != sum ? 1.0f / sum : 0.0f;
+            // ---- O / sum; the sum of a row that saw no key is 0
+            const float scale = sum != 0 ? 1.0f / sum : 0.0f;
             const uint64_t scale2 = Both(scale, scale);
             T *out = (T *)a.out + ((size_t)w.q0 + token) * a.outStride[0] + (size_t)head * a.outStride[1];
             uint64_t odd = 0;  // stays 0 as long as what is added is 0 times something finite
@@ -746,7 +747,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                 }
             }
             if (a.lse != nullptr && valid) {
-                a.lse[((size_t)w.q0 + token) * a.kvHeads * a.group + head] = top == -INFINITY ? -INFINITY : top * factor * kLn2 + logf(sum);
+                a.lse[((size_t)w.q0 + token) * a.kvHeads * a.group + head] = top * factor * kLn2 + logf(sum);
             }
             const float2 any = Apart(odd);
             unsigned again = __ballot_sync(~0u, !(any.x + any.y == 0.0f) && valid);
