@@ -135,51 +135,5 @@ __device__ __forceinline__ float Exp2(float x)
     return r;
 }
 
-// One row of attention by one warp, key by key: for rows whose result is not finite. In a tile product a masked key counts 0 * v, which is
-// not 0 where v is infinite or NaN; here only the keys below `seen` are touched. q: the row's query, out: its place.
-template <typename T, int D>
-__device__ __noinline__ void AttendRow(const T *q, const T *k, long long kStep, const T *v, long long vStep, int seen, float factor, T *out, float *lse)
-{
-    constexpr int kMine = D / 64;  // pairs of columns of a lane
-    const int lane = threadIdx.x & 31;
-    float x[2 * kMine], acc[2 * kMine], top = -INFINITY, sum = 0;
-#pragma unroll
-    for (int i = 0; i < kMine; i++) {
-        const float2 p = Unpack2<T>(*(const uint32_t *)(q + i * 64 + lane * 2));
-        x[2 * i] = p.x, x[2 * i + 1] = p.y;
-        acc[2 * i] = acc[2 * i + 1] = 0;
-    }
-    for (int j = 0; j < seen; j++) {
-        float s = 0;
-#pragma unroll
-        for (int i = 0; i < kMine; i++) {
-            const float2 p = Unpack2<T>(*(const uint32_t *)(k + j * kStep + i * 64 + lane * 2));
-            s += x[2 * i] * p.x + x[2 * i + 1] * p.y;
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-            s += __shfl_xor_sync(~0u, s, d);
-        }
-        s *= factor;
-        const float best = fmaxf(top, s), base = best == -INFINITY ? 0.0f : best, shrink = Exp2(top - base), p = Exp2(s - base);
-        top = best;
-        sum = sum * shrink + p;
-#pragma unroll
-        for (int i = 0; i < kMine; i++) {
-            const float2 y = Unpack2<T>(*(const uint32_t *)(v + j * vStep + i * 64 + lane * 2));
-            acc[2 * i] = acc[2 * i] * shrink + p * y.x;
-            acc[2 * i + 1] = acc[2 * i + 1] * shrink + p * y.y;
-        }
-    }
-    const float scale = sum != 0 ? 1.0f / sum : 0.0f;
-#pragma unroll
-    for (int i = 0; i < kMine; i++) {
-        *(uint32_t *)(out + i * 64 + lane * 2) = Pack2<T>(acc[2 * i] * scale, acc[2 * i + 1] * scale);
-    }
-    if (lse != nullptr && lane == 0) {
-        *lse = top * kLn2 + logf(sum);
-    }
-}
-
 }  // namespace attn
 }  // namespace mf

@@ -13,13 +13,18 @@
 //                    the P that the second overwrites, and the tensor core takes them in order.
 //   warp 9           TMA: both Q tiles, then keys and values in turn through a ring of stages.
 //   warp 10          takes the CTA's next two row tiles from the work that is left, while the present ones are computed.
+//   warp 11          takes infinities and NaN out of the values of keys that some rows must not see, in units that are done once more for them.
 //
 // The reference m only follows the maximum where a weight would pass 2^8 (fp16: 2^14); then the row's O is scaled in TMEM. That is rare, so no
 // warps are kept for it. The S barrier of a key tile stands for the completion of all MMAs before it, so O is at rest when its S arrives.
 //
 // p is rounded to the operands' type for the second product (the tensor core wants one type for both); the sum is taken before
-// that, all sums and O are fp32. A masked key counts 0 * v in a tile product, which is not 0 where v is infinite or NaN: a row whose result is not finite
-// is computed again key by key. All waits are bounded; one that runs out sets the status, and the CTA drains and leaves.
+// that, all sums and O are fp32. All waits are bounded; one that runs out sets the status, and the CTA drains and leaves.
+//
+// A masked key counts 0 * v in a tile product, which is not 0 where v is infinite or NaN. Only the last one to three key tiles of a unit of work hold keys
+// that not all of its rows see. Where a row of such a unit comes out infinite or NaN, the unit is done once more, clean: warp 11 makes what is infinite or
+// NaN among the values of those keys 0 in shared memory before the product, and gives it back to the rows that see it behind it. What all rows see is left
+// to the product. So such a unit takes twice its time, and the others 1 to 2 % for being ready for it (cleaning all of them: 3 to 11 %).
 #include <cuda.h>
 
 #include <type_traits>
@@ -46,6 +51,7 @@ constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;
 struct Work {
     int q0, rows, t0;   // first query row of the sequence, their number, first token of the tiles
     int k0, keys, n;    // first key, their number, key tiles to go through; n < 0: no more work
+    int sure, clean;    // keys that all rows see; whether the values of the others are to be cleaned
     int kvh, h0;
 };
 
@@ -55,13 +61,17 @@ struct Shared {
     static constexpr uint32_t kTileBytes = (D / 64) * kHalf;
     unsigned char q[2][kTileBytes];
     unsigned char kv[kStages][kTileBytes];
-    uint64_t qFull, qEmpty, kvFull[kStages], kvEmpty[kStages], sFull[2], pFull[2], pRest[2], oFull[2], workFull[2], workEmpty[2];
+    uint64_t qFull, qEmpty, kvFull[kStages], kvEmpty[kStages], kvRaw[kStages], sFull[2], pFull[2], pRest[2], oFull[2], workFull[2], workEmpty[2];
     uint4 claim;  // the answer to Claim()
     uint64_t claimed;
-    Work work[2];
+    Work work[2], late;  // late: done clean, to get back what was taken out
+    int odd[2];  // a row of the work came out infinite or NaN
     uint32_t tmem;
     int abortFlag;
 };
+
+// The first key tile that has to be cleaned.
+__device__ __forceinline__ int CutTile(const Work &w) { return w.clean ? w.sure / kTile : w.n; }
 
 struct Params {
     mf_prefill_attention_args_t a;
@@ -183,8 +193,7 @@ __device__ __forceinline__ int ClaimedCta(const uint4 *answer)
     return x;
 }
 
-// A row that is computed again key by key (AttendRow) holds its CTA up for as long as that takes, 2.5 seconds for a million keys, so the waits in this kernel
-// have a minute.
+// Some waits last as long as a unit of work, 14 ns a key: a minute is enough for any number of keys.
 __device__ __forceinline__ bool Wait(uint64_t *bar, uint32_t parity, volatile int *abortFlag) { return MbarWaitWarp(bar, parity, abortFlag, 60000000000ull); }
 
 // Sequence b's query rows and keys, as far as there are tokens; none where the offsets descend or begin outside.
@@ -306,6 +315,91 @@ struct Ranking {
     }
 };
 
+template <typename T>
+struct Bits {
+    static constexpr uint32_t kExponent = Bf16<T>::value ? 0x7f80u : 0x7c00u;  // all set: infinite or NaN
+    static __device__ __forceinline__ bool Finite(uint32_t x) { return (x & kExponent) != kExponent; }
+};
+// The larger absolute values of two pairs, NaN if one is; the signs mean nothing.
+template <typename T>
+__device__ __forceinline__ uint32_t MaxAbs2(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    if (Bf16<T>::value) {
+        asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    } else {
+        asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    }
+    return r;
+}
+
+// What is infinite or NaN among the values of the keys from r0 on of a tile in shared memory becomes 0. Whole warp.
+template <typename T, int D>
+__device__ __noinline__ void Clean(unsigned char *tile, int r0)
+{
+    for (int c = 0; c < D / 64; c++) {
+        uint4 *at = (uint4 *)(tile + c * kHalf);
+        for (int i = r0 * 8 + (threadIdx.x & 31); i < kTile * 8; i += 32) {  // 128 bytes to a key
+            uint4 x = at[i];
+            uint32_t *const word[4] = {&x.x, &x.y, &x.z, &x.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                *word[e] &= (Bits<T>::Finite(*word[e]) ? 0xffffu : 0) | (Bits<T>::Finite(*word[e] >> 16) ? 0xffff0000u : 0);
+            }
+            at[i] = x;
+        }
+    }
+    FenceProxyAsyncShared();  // the tensor core reads what was written here
+}
+
+// Gives the rows of a unit of work back what Clean() has taken out of values that they see, those of the keys [sure, limit of the row). What is added to an
+// element of O is infinite or NaN, so it may as well be added to the result. A lane has two columns at a time, and four rows' loads in flight: with eight the
+// kernel has to spill registers, and takes 3 % longer.
+template <typename T, int D>
+__device__ __noinline__ void Restore(const Params &p, const Work &w)
+{
+    const mf_prefill_attention_args_t &a = p.a;
+    const int lane = threadIdx.x & 31, rows = min(p.tokens, w.rows - w.t0) * p.pack, past = w.keys - w.rows + w.t0 + 1;
+    const int see = a.causal ? min(p.tokens, w.rows - w.t0) + past - 1 : w.keys;
+    for (int turn = 0; turn < 3 * (D / 64); turn++) {
+        const int kind = turn % 3, c = turn / 3 * 64 + lane * 2;
+        const float more = kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
+        int first[2] = {see, see};  // the first key where each column is that
+        const T *v = (const T *)a.v + (size_t)w.k0 * a.vStride[0] + (size_t)w.kvh * a.vStride[1] + c;
+#pragma unroll 4
+        for (int j = see - 1; j >= w.sure; j--) {
+            const float2 x = Unpack2<T>(*(const uint32_t *)(v + j * a.vStride[0]));
+            first[0] = kind == 0 ? (x.x != x.x ? j : first[0]) : x.x == more ? j : first[0];
+            first[1] = kind == 0 ? (x.y != x.y ? j : first[1]) : x.y == more ? j : first[1];
+        }
+        const int least = min(first[0], first[1]);
+        if (__all_sync(~0u, least == see)) {
+            continue;
+        }
+        T *out = (T *)a.out + ((size_t)w.q0 + w.t0) * a.outStride[0] + (size_t)w.h0 * a.outStride[1] + c;
+        constexpr int kAhead = 4;
+        for (int r0 = 0; r0 < rows; r0 += kAhead) {
+            uint32_t was[kAhead];
+#pragma unroll
+            for (int store = 0; store < 2; store++) {
+#pragma unroll
+                for (int u = 0; u < kAhead; u++) {
+                    const int t = (r0 + u) / p.pack, limit = r0 + u >= rows ? least : a.causal ? min(w.keys, t + past) : w.keys;
+                    uint32_t *const at = (uint32_t *)(out + t * a.outStride[0] + (r0 + u) % p.pack * a.outStride[1]);
+                    if (limit > least) {
+                        if (store) {
+                            const float2 y = Unpack2<T>(was[u]);
+                            *at = Pack2<T>(limit > first[0] ? y.x + more : y.x, limit > first[1] ? y.y + more : y.y);
+                        } else {
+                            was[u] = *at;
+                        }
+                    }
+                }
+            }
+        }
+    }
+}
+
 // A warp's view of the work list: the next two row tiles, or false at its end.
 template <int D>
 struct Worker {
@@ -343,6 +437,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
         for (int i = 0; i < X::kStages; i++) {
             MbarInit(&s.kvFull[i], 1);
             MbarInit(&s.kvEmpty[i], 1);
+            MbarInit(&s.kvRaw[i], 1);
         }
         for (int i = 0; i < 2; i++) {
             MbarInit(&s.sFull[i], 1);
@@ -350,7 +445,8 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
             MbarInit(&s.pRest[i], 4);
             MbarInit(&s.oFull[i], 1);
             MbarInit(&s.workFull[i], 1);
-            MbarInit(&s.workEmpty[i], 10);
+            MbarInit(&s.workEmpty[i], 11);
+            s.odd[i] = 0;
         }
         MbarInit(&s.claimed, 1);
         s.abortFlag = 0;
@@ -379,28 +475,59 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
             if (a.B <= kRanked) {
                 ranking.Begin(p);
             }
+            const Work none = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
             int k = 0, unit = (int)blockIdx.x;
-            for (uint32_t claims = 0;; claims++) {
+            // Hands a work out and waits until all warps have taken it: so the other place is free, and they are done with the one before, of which it is known
+            // now whether it came out finite.
+            bool ok = true, odd = false;
+            auto put = [&](const Work &w) {
+                if (ok) {
+                    if (lane == 0) {
+                        s.work[k & 1] = w;
+                        s.odd[k & 1] = 0;
+                        MbarArrive(&s.workFull[k & 1]);
+                    }
+                    ok = Wait(&s.workEmpty[k & 1], (k >> 1) & 1, abortFlag);
+                    k++;
+                    odd = ok && __shfl_sync(~0u, s.odd[k & 1], 0) != 0;
+                }
+            };
+            for (uint32_t claims = 0; ok; claims++) {
                 const bool end = unit < 0;
                 const int number = unit / p.headTiles, ht = unit - number * p.headTiles;
-                Work w = {0, 0, 0, 0, 0, -1, 0, 0};
+                Work w = none;
                 const bool there = !end && (a.B <= kRanked ? ranking.Find(p, number, w) : Numbered(p, number, w));
                 if (there) {
                     const int see = a.causal ? min(w.keys, min(w.rows, w.t0 + p.tokens) + w.keys - w.rows) : w.keys;
-                    w.n = see > 0 ? (see + kTile - 1) / kTile : 0;
+                    w.n = see > 0 ? (see - 1) / kTile + 1 : 0;
+                    w.sure = a.causal ? max(0, min(w.keys, w.t0 + w.keys - w.rows + 1)) : w.keys;
+                    w.clean = 0;
                     const int perKv = a.group / p.pack;
                     w.kvh = ht / perKv;
                     w.h0 = w.kvh * a.group + (ht % perKv) * p.pack;
                 }
-                if (there || end) {
-                    if (lane == 0) {
-                        s.work[k & 1] = w;
+                if (there || end) {  // at the end one without rows: then it is known of the last one, too
+                    put(w);
+                    if (odd) {
+                        Work again = s.work[k & 1], last = s.work[(k + 1) & 1];  // the one before w, and w
+                        __syncwarp();
+                        for (bool more = true; ok && more && !again.clean && again.sure / kTile < again.n; again = last, last = none) {
+                            again.clean = 1;
+                            put(again);
+                            more = odd;  // of `last`
+                            put(none);   // when the warps have taken what comes behind this one, they are done with the clean one
+                        }
+                    }
+                }
+                if (end) {
+                    if (lane == 0 && ok) {
+                        s.work[k & 1].n = -1;
                         MbarArrive(&s.workFull[k & 1]);
                     }
-                    if (end || !Wait(&s.workEmpty[k & 1], (k >> 1) & 1, abortFlag)) {  // so the other place is free, too
-                        break;
-                    }
-                    k++;
+                    break;
+                }
+                if (!ok) {
+                    break;
                 }
                 if (lane == 0) {
                     MbarExpectTx(&s.claimed, 16);
@@ -419,7 +546,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
             const bool elected = ElectOne();
             Worker<D> worker;
             Work w;
-            uint32_t st = 0, ph = 0, qPh = 0;
+            uint32_t st = 0, ph = 0, qPh = 0, raw = 0, rawPh = 0;
             long long issued = 0;
             bool ok = true, qOpen = false;
             while (ok && worker.Next(s, abortFlag, w)) {
@@ -441,17 +568,22 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                 }
                 qOpen = true;
                 qPh ^= 1;
+                const int cut = CutTile(w);
                 for (int i = 0; i < 2 * w.n; i++) {
                     ok = Wait(&s.kvEmpty[st], ph ^ 1, abortFlag);
                     if (!ok) {
                         break;
                     }
+                    const bool dirty = (i & 1) != 0 && (i >> 1) >= cut;  // goes to warp 11 first
+                    uint64_t *const full = dirty ? &s.kvRaw[st] : &s.kvFull[st];
                     if (elected) {
-                        MbarExpectTx(&s.kvFull[st], X::kTileBytes);
+                        MbarExpectTx(full, X::kTileBytes);
                         for (int c = 0; c < D / 64; c++) {
-                            TmaLoad3D(s.kv[st] + c * kHalf, i & 1 ? &mapV : &mapK, &s.kvFull[st], c * 64, w.kvh, w.k0 + (i >> 1) * kTile);
+                            TmaLoad3D(s.kv[st] + c * kHalf, i & 1 ? &mapV : &mapK, full, c * 64, w.kvh, w.k0 + (i >> 1) * kTile);
                         }
                     }
+                    raw = (raw & ~(1u << st)) | (dirty ? 1u << st : 0);
+                    rawPh ^= dirty ? 1u << st : 0;
                     issued++;
                     if (++st == X::kStages) {
                         st = 0;
@@ -465,7 +597,58 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                     MbarWaitBounded(&s.qFull, qPh ^ 1, &own);
                 }
                 for (long long i = issued > X::kStages ? issued - X::kStages : 0; i < issued; i++) {
-                    MbarWaitBounded(&s.kvFull[i % X::kStages], (uint32_t)(i / X::kStages) & 1, &own);
+                    const uint32_t at = (uint32_t)(i % X::kStages);
+                    if (raw >> at & 1) {
+                        MbarWaitBounded(&s.kvRaw[at], (rawPh >> at & 1) ^ 1, &own);
+                    } else {
+                        MbarWaitBounded(&s.kvFull[at], (uint32_t)(i / X::kStages) & 1, &own);
+                    }
+                }
+            }
+        } else if (warp == 11) {
+            // ------------------------------------------------------------------ values that are not finite
+            // Such a tile's arrival is counted on kvRaw, which has a phase for each time that its stage holds one; kvFull is completed here, when it is clean. So
+            // the MMA warp knows nothing of this: with one more barrier in its loop, never waited for, prompts took 1 to 2 % longer.
+            Worker<D> worker;
+            Work taken;
+            uint32_t st = 0, rawPh = 0;
+            int lateAt = -2;
+            auto move = [&](uint32_t by) { st = (st + by) % X::kStages; };
+            bool ok = true;
+            for (bool more = true; more;) {
+                more = worker.Next(s, abortFlag, taken);
+                if (*abortFlag != 0) {
+                    break;
+                }
+                if (worker.k == lateAt + 2) {  // the other warps have taken the one behind it, so its rows are stored
+                    Restore<T, D>(p, s.late);
+                }
+                if (!more) {
+                    break;
+                }
+                const Work &w = s.work[(worker.k - 1) & 1];  // stays until this warp has taken the next one
+                const int cut = CutTile(w);
+                move(2 * cut);
+                for (int j = cut; j < w.n; j++) {
+                    move(1);
+                    ok = Wait(&s.kvRaw[st], rawPh >> st & 1, abortFlag);
+                    if (!ok) {
+                        break;
+                    }
+                    rawPh ^= 1u << st;
+                    Clean<T, D>(s.kv[st], max(0, w.sure - j * kTile));
+                    __syncwarp();
+                    if (lane == 0) {
+                        MbarArrive(&s.kvFull[st]);
+                    }
+                    move(1);
+                }
+                if (w.clean) {
+                    if (lane == 0) {
+                        s.late = w;
+                    }
+                    __syncwarp();
+                    lateAt = worker.k;
                 }
             }
         } else if (warp == 8) {
@@ -683,7 +866,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
         uint32_t sPh = 0, oPh = 0;
         bool ok = true;
         while (ok && worker.Next(s, abortFlag, w)) {
-            if (i == 1 && w.t0 + half >= w.rows) {
+            if (w.t0 + i * half >= w.rows) {
                 continue;
             }
             const int token = w.t0 + rowToken, past = w.keys - w.rows, head = w.h0 + rowHead;
@@ -746,20 +929,12 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
                     }
                 }
             }
+            const float2 any = Apart(odd);
+            if (!(any.x + any.y == 0.0f) && valid) {
+                s.odd[(worker.k - 1) & 1] = 1;
+            }
             if (a.lse != nullptr && valid) {
                 a.lse[((size_t)w.q0 + token) * a.kvHeads * a.group + head] = top * factor * kLn2 + logf(sum);
-            }
-            const float2 any = Apart(odd);
-            unsigned again = __ballot_sync(~0u, !(any.x + any.y == 0.0f) && valid);
-            while (again != 0) {
-                const int r = (warp & 3) * 32 + __ffs(again) - 1, t = w.t0 + i * half + r / p.pack, h = w.h0 + r % p.pack;
-                again &= again - 1;
-                const size_t q = (size_t)(w.q0 + t);
-                AttendRow<T, D>((const T *)a.q + q * a.qStride[0] + (size_t)h * a.qStride[1],
-                                (const T *)a.k + (size_t)w.k0 * a.kStride[0] + (size_t)w.kvh * a.kStride[1], a.kStride[0],
-                                (const T *)a.v + (size_t)w.k0 * a.vStride[0] + (size_t)w.kvh * a.vStride[1], a.vStride[0],
-                                a.causal ? min(w.keys, t + past + 1) : w.keys, factor, (T *)a.out + q * a.outStride[0] + (size_t)h * a.outStride[1],
-                                a.lse != nullptr ? a.lse + q * a.kvHeads * a.group + h : nullptr);
             }
         }
     }
