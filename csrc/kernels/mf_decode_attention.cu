@@ -822,7 +822,7 @@ extern "C" int mf_k_decode_attention(const mf_decode_attention_args_t *args, int
     const int ctas = Ctas(a.B, a.kvHeads, a.group, capacity);
     if (capacity <= kWholeKeys) {
         a.workspace = a.marks = nullptr;
-    } else if (a.workspace == nullptr) {
+    } else if (a.workspace == nullptr || a.workspaceBytes < mf_k_decode_attention_workspace(a.B, a.kvHeads, a.group, D, capacity)) {
         return MF_K_INVALID;
     } else {
         a.marks = (unsigned char *)a.workspace + PartialBytes(ctas, a.group, D);

@@ -264,7 +264,7 @@ typedef struct {
     void *out;
     float *lse;
     int *status;
-    void *workspace;  // mf_k_decode_attention_workspace() bytes of this call's own (NULL if that says 0)
+    void *workspace;  // mf_k_decode_attention_workspace() bytes of this call's own, on the GPU of the call (NULL if that says 0)
     void *marks;      // set by the launcher
     long long qStride[2];
     long long outStride[2];
@@ -274,6 +274,7 @@ typedef struct {
     float scale;
     unsigned pageMagic;  // set by the launcher
     int pageShift;       // set by the launcher
+    size_t workspaceBytes;  // fewer than the call needs are refused
 } mf_decode_attention_args_t;
 size_t mf_k_decode_attention_workspace(int B, int kvHeads, int group, int D, long long capacity);
 int mf_k_decode_attention(const mf_decode_attention_args_t *args, int D, int qType, int cacheType, mf_stream_t stream);

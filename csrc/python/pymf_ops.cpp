@@ -334,7 +334,7 @@ void BindOps(py::module_ &m)
             return mf_k_decode_attention_workspace(p.a.B, p.a.kvHeads, p.a.group, p.dim, (long long)p.a.tableWidth * p.a.pageSize);
         })
         .def("run", [](const DecodePlan &p, uint64_t q, uint64_t k, uint64_t v, uint64_t out, uint64_t table, uint64_t lengths, uint64_t rows, uint64_t kScale,
-                       uint64_t vScale, uint64_t lse, uint64_t status, uint64_t workspace, float scale, uint64_t stream) {
+                       uint64_t vScale, uint64_t lse, uint64_t status, uint64_t workspace, uint64_t workspaceBytes, float scale, uint64_t stream) {
             mf_decode_attention_args_t a = p.a;
             a.q = (const void *)q;
             a.k = (const void *)k;
@@ -348,6 +348,7 @@ void BindOps(py::module_ &m)
             a.lse = (float *)lse;
             a.status = (int *)status;
             a.workspace = (void *)workspace;
+            a.workspaceBytes = workspaceBytes;
             a.scale = scale;
             return mf_k_decode_attention(&a, p.dim, p.qType, p.cacheType, (mf_stream_t)stream);
         });

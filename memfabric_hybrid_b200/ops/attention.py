@@ -169,7 +169,9 @@ def _plan_decode(key, q, k_pages, v_pages, table, lengths, rows, k_scale, v_scal
            status=status)
     native = _ops.DecodePlan(*qs, *os, *step, table.stride(0), B, kv_heads, heads // kv_heads, page_size, pages, table.shape[1], table.shape[0], dim, q_type,
                              cache_type)
-    return _decode_plans.put(key, (native, (native.workspace() + 3) // 4, dim ** -0.5))
+    with launch_on(q.device.index, None):  # its size goes by the GPU that the call runs on, whichever is the current one
+        words = (native.workspace() + 3) // 4
+    return _decode_plans.put(key, (native, words, dim ** -0.5))
 
 
 def decode_attention(q, k_pages, v_pages, table, lengths, *, rows=None, scale=None, k_scale=None, v_scale=None, out=None, lse=None, status=None,
@@ -209,7 +211,7 @@ def decode_attention(q, k_pages, v_pages, table, lengths, *, rows=None, scale=No
             raise ValueError(_misaligned)
         rc = native.run(*at, table.data_ptr(), lengths.data_ptr(), 0 if rows is None else rows.data_ptr(), 0 if k_scale is None else k_scale.data_ptr(),
                         0 if v_scale is None else v_scale.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if status is None else status.data_ptr(),
-                        0 if ws is None else ws.data_ptr(), factor, current_stream_handle())
+                        0 if ws is None else ws.data_ptr(), 4 * words, factor, current_stream_handle())
     if rc != 0:
         raise RuntimeError(f"decode_attention launch failed ({rc})")
     return (out, lse) if with_lse else out
