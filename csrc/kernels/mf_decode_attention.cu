@@ -19,9 +19,10 @@
 // head lie in the lanes that hold its results. The reference of the exponentials follows the maximum only where a weight
 // would pass 2^8 (fp16: 2^14): most tiles need one vote for it, no shuffles and no scaling of the output.
 //
-// 8-bit caches are widened to fp16, which holds every e4m3 value; the query is scaled by a power of two per head so that it fits fp16
-// without loss. p is rounded to the cache's type (fp16 for 8-bit caches) for the second product, as the tensor cores want equal
-// types; the sum is taken before that rounding, all sums in fp32.
+// 8-bit caches are widened to fp16, which holds every e4m3 value. The query is scaled by a power of two per head, its largest element into
+// [2^14, 2^15): bf16 elements down to 2^-31 of that keep all their bits, smaller ones err by 2^-39 of it at most (half of fp16's least step).
+// p is rounded to the cache's type (fp16 for 8-bit caches) for the second product, as the tensor cores want equal types; the sum is taken
+// before that rounding, all sums in fp32.
 #include "mf/device/mf_shm_device.cuh"
 #include "mf_attention.cuh"
 #include "mf_kernels.h"
@@ -375,10 +376,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode
                     }
                     biggest = fmaxf(biggest, __shfl_xor_sync(~0u, biggest, 1));
                     biggest = fmaxf(biggest, __shfl_xor_sync(~0u, biggest, 2));
-                    int e = (int)(__float_as_uint(biggest) >> 23) - 127;  // its exponent: scaled values lie below two
-                    e = biggest == 0 || e > 126 ? 0 : e < -100 ? -100 : e;
-                    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                    up = __uint_as_float((uint32_t)(127 + e) << 23);
+                    int e = (int)(__float_as_uint(biggest) >> 23) - 127;  // its exponent: scaled values lie below 2^15
+                    e = biggest == 0 || e > 127 ? 0 : e < -100 ? -100 : e;
+                    const float down = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+                    up = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
 #pragma unroll
                     for (int s = 0; s < kSteps; s++) {
                         const float2 x = Unpack2<Q>(q[t][s][0]), y = Unpack2<Q>(q[t][s][1]);
