@@ -13,6 +13,7 @@ import contextlib
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _loader  # noqa: F401
 from .._loader import _pymf
@@ -70,8 +71,12 @@ def launch_on(device, stream):
 def no_gradient(*tensors):
     if torch.is_grad_enabled():
         for t in tensors:
-            if t.requires_grad:
+            if t is not None and t.requires_grad:
                 raise RuntimeError("this operator has no backward pass: call it under torch.no_grad(), or detach its inputs")
+    if forward_ad._current_level >= 0:  # within a dual_level()
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("this operator has no forward-mode derivative: call it with the primals (torch.autograd.forward_ad.unpack_dual)")
 
 
 def int32(name, t, dims):
@@ -188,10 +193,10 @@ def decode_attention(q, k_pages, v_pages, table, lengths, *, rows=None, scale=No
 
     status: int32 tensor of one element, receives MF_DEV_ERR_BOUNDS (2) where a length reaches a page number that does not exist (its
     keys and values then count as zeros) or rows names no sequence (which then has no tokens)."""
-    no_gradient(q, k_pages, v_pages)
     with_lse = lse is not None and lse is not False
     if lse is True or lse is False:
         lse = None
+    no_gradient(q, k_pages, v_pages, k_scale, v_scale, out, lse)
     # the required tensors one by one and the others by name, as a call takes no longer than a few of these look-ups
     key = (q.shape, q.stride(), q.dtype, q.get_device(), k_pages.shape, k_pages.stride(), k_pages.dtype, k_pages.get_device(), v_pages.shape, v_pages.stride(),
            v_pages.dtype, v_pages.get_device(), table.shape, table.stride(), table.dtype, table.get_device(), lengths.shape, lengths.stride(), lengths.dtype,
@@ -253,10 +258,10 @@ def prefill_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, out=
     Returns out [tokens, heads, dim]; with lse=True (or a tensor for it) also the logarithm of the sum of exponentials, fp32
     [tokens, heads]. Rows that see no key give zeros and -inf; rows that belong to no sequence are left as they are. out must not overlap the
     inputs. status: int32 tensor of one element, receives GEMM_PIPELINE_EXPIRED (3) if a bounded wait inside the kernel ran out."""
-    no_gradient(q, k, v)
     with_lse = lse is not None and lse is not False
     if lse is True or lse is False:
         lse = None
+    no_gradient(q, k, v, out, lse)
     cu_k = cu_q if cu_k is None else cu_k
     key = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype, v.get_device(), cu_q.shape,
            cu_q.stride(), cu_q.dtype, cu_q.get_device(), cu_k.shape, cu_k.stride(), cu_k.dtype, cu_k.get_device(),

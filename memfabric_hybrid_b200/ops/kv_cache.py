@@ -133,7 +133,7 @@ class PagedKVCache:
         plan = self._writes.get(key) or self._writes.put(key, self._plan_write(k, v, slots, k_scale, v_scale))
         if not 0 <= layer < self.layers:
             raise ValueError(f"there are {self.layers} layers")
-        no_gradient(k, v)
+        no_gradient(k, v, k_scale, v_scale)
         with launch_on(self._device.index, stream):
             at = k.data_ptr(), v.data_ptr()
             if (at[0] | at[1]) & 15:

@@ -3,8 +3,10 @@ import contextlib
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from memfabric_hybrid_b200.ops import attention as A
+from memfabric_hybrid_b200.ops.kv_cache import PagedKVCache
 
 BF = torch.bfloat16
 
@@ -50,3 +52,42 @@ def test_a_workspace_that_is_too_small_is_refused(dim):
     for given in (0, 4, need - 4):
         # refused before anything is launched: the addresses are none
         assert plan.run(0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 4096, given, 1.0, 0) == -2
+
+
+def _decode(**kw):
+    a = {"q": torch.zeros(3, 8, 64, dtype=BF), "k": torch.zeros(5, 2, 16, 64).to(torch.float8_e4m3fn), "k_scale": torch.ones(2), "v_scale": torch.ones(2)} | kw
+    k = a.pop("k")
+    return A.decode_attention(a.pop("q"), k, k, torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), **a)
+
+
+def _prefill(**kw):
+    a = {"q": torch.zeros(10, 8, 64, dtype=BF), "k": torch.zeros(10, 2, 64, dtype=BF), "v": torch.zeros(10, 2, 64, dtype=BF)} | kw
+    return A.prefill_attention(a.pop("q"), a.pop("k"), a.pop("v"), torch.zeros(3, dtype=torch.int32), **a)
+
+
+def _write(**kw):
+    cache = PagedKVCache.__new__(PagedKVCache)  # without a GPU there is none
+    cache.layers, cache._writes = 1, A.Plans()
+    cache._plan_write = lambda *args: (0,)
+    a = {"k": torch.zeros(10, 2, 64, dtype=BF), "v": torch.zeros(10, 2, 64, dtype=BF), "k_scale": torch.ones(2), "v_scale": torch.ones(2)} | kw
+    cache.write(0, a.pop("k"), a.pop("v"), torch.zeros(10, dtype=torch.int64), **a)
+
+
+CALLS = [(_decode, "q", (3, 8, 64), BF), (_decode, "k_scale", (2,), torch.float32), (_decode, "v_scale", (2,), torch.float32), (_decode, "out", (3, 8, 64), BF),
+         (_decode, "lse", (3, 8), torch.float32), (_prefill, "q", (10, 8, 64), BF), (_prefill, "k", (10, 2, 64), BF), (_prefill, "v", (10, 2, 64), BF),
+         (_prefill, "out", (10, 8, 64), BF), (_prefill, "lse", (10, 8), torch.float32), (_write, "k", (10, 2, 64), BF), (_write, "v", (10, 2, 64), BF),
+         (_write, "k_scale", (2,), torch.float32), (_write, "v_scale", (2,), torch.float32)]
+
+
+@pytest.mark.parametrize("call,name,shape,dtype", CALLS)
+def test_whatever_wants_a_gradient_is_refused(call, name, shape, dtype):
+    with pytest.raises(RuntimeError, match="backward"):
+        call(**{name: torch.zeros(shape, dtype=dtype, requires_grad=True)})
+
+
+@pytest.mark.parametrize("call,name,shape,dtype", CALLS)
+def test_tangents_are_not_dropped(call, name, shape, dtype):
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(torch.zeros(shape, dtype=dtype), torch.ones(shape, dtype=dtype))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            call(**{name: x})
