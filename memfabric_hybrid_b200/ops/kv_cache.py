@@ -80,10 +80,13 @@ class PagedKVCache:
         return self.data.data_ptr() + (layer * self.pages + page) * n, n
 
     def check_status(self) -> int:
-        """0, or MF_DEV_ERR_BOUNDS (2) if a call since the last check was refused on the device, wholly or in part. Waits for the GPU."""
+        """0, or MF_DEV_ERR_BOUNDS (2) if a call since the last check was refused on the device, wholly or in part. Waits for the GPU, whatever
+        streams the calls were given."""
+        torch.cuda.synchronize(self._device)  # the calls may have been given other streams than the current one
         s = int(self.status.item())
         if s:
             self.status.zero_()
+            torch.cuda.current_stream(self._device).synchronize()  # before another stream's next call
         return s
 
     def _request(self, name, t):
