@@ -10,7 +10,6 @@ statistics in fp32. All tensors are on one GPU; lengths and offsets stay on the 
 from __future__ import annotations
 
 import contextlib
-import math
 
 import torch
 from torch.autograd import forward_ad
@@ -135,8 +134,8 @@ def _check_result(out, like_shape, like_dtype, lse, lse_shape):
 def _scale(scale, dim):
     if scale is None:
         return dim ** -0.5
-    if not (scale > 0 and math.isfinite(scale)):
-        raise ValueError("scale must be positive and finite")
+    if not 2.0 ** -125 <= scale <= 2.0 ** 127:  # times log2(e), and 6 divided by that, are fp32 numbers in the kernels
+        raise ValueError("scale must be positive, from 2^-125 to 2^127")
     return float(scale)
 
 
@@ -186,10 +185,10 @@ def decode_attention(q, k_pages, v_pages, table, lengths, *, rows=None, scale=No
     q [B, heads, dim]; k_pages, v_pages [pages, kv_heads, page_size, dim] (any strides, the same for both; pass `.transpose(1, 2)` of pages that
     are kept token by token), heads a multiple of kv_heads; table int32 [seqs, width]: the pages of each sequence; lengths int32 [seqs]: its
     tokens (no more than width * page_size count). rows int32 [B]: the sequence of each query, by default the first B. Pages in q's type, or
-    float8_e4m3fn with k_scale, v_scale fp32 [kv_heads] (value = e4m3 * scale). scale: of the logits, 1 / sqrt(dim) by default. Returns out
-    [B, heads, dim]; with lse=True (or a tensor for it) also the logarithm of the sum of exponentials, fp32 [B, heads]. A sequence without
-    tokens gives zeros and -inf. What lies in a page behind a sequence's length does not matter. The last bits of a row may depend
-    on what else is in the batch (that decides where long rows are cut), and on nothing else. out must not overlap the inputs.
+    float8_e4m3fn with k_scale, v_scale fp32 [kv_heads] (value = e4m3 * scale). scale: of the logits, 2^-125 to 2^127, 1 / sqrt(dim) by
+    default. Returns out [B, heads, dim]; with lse=True (or a tensor for it) also the logarithm of the sum of exponentials, fp32 [B, heads].
+    A sequence without tokens gives zeros and -inf. What lies in a page behind a sequence's length does not matter. The last bits of a row
+    may depend on what else is in the batch (that decides where long rows are cut), and on nothing else. out must not overlap the inputs.
 
     status: int32 tensor of one element, receives MF_DEV_ERR_BOUNDS (2) where a length reaches a page number that does not exist (its
     keys and values then count as zeros) or rows names no sequence (which then has no tokens)."""
@@ -253,7 +252,7 @@ def prefill_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, out=
     """Attention of packed prompts. q [tokens, heads, dim], k and v [keys, kv_heads, dim] (any strides, rows contiguous, not expanded), heads a multiple
     of kv_heads; cu_q int32 [B + 1]: the rows of sequence b are cu_q[b] to cu_q[b + 1], ascending from 0 or more; cu_k the same for keys,
     by default cu_q. With `causal` the last row of a sequence sees all of its keys, each row before it one less: a chunk of a prompt is given as
-    its rows with all keys up to its end. scale: of the logits, 1 / sqrt(dim) by default.
+    its rows with all keys up to its end. scale: of the logits, 2^-125 to 2^127, 1 / sqrt(dim) by default.
 
     Returns out [tokens, heads, dim]; with lse=True (or a tensor for it) also the logarithm of the sum of exponentials, fp32
     [tokens, heads]. Rows that see no key give zeros and -inf; rows that belong to no sequence are left as they are. out must not overlap the

@@ -91,3 +91,15 @@ def test_tangents_are_not_dropped(call, name, shape, dtype):
         x = forward_ad.make_dual(torch.zeros(shape, dtype=dtype), torch.ones(shape, dtype=dtype))
         with pytest.raises(RuntimeError, match="forward-mode"):
             call(**{name: x})
+
+
+@pytest.mark.parametrize("scale", [1e39, 1.8e38, 2.0 ** 127 * 1.01, 1e-38, 1e-45, 1e-50])
+@pytest.mark.parametrize("call", [_decode, _prefill])
+def test_scales_that_fp32_does_not_hold_are_refused(call, scale):
+    """As fp32 numbers, with the factor to powers of two and its inverse: infinite, 0 or without all their bits."""
+    with pytest.raises(ValueError, match="scale must"):
+        A._scale(scale, 64)
+    for fine in (2.0 ** 127, 2.0 ** -125, 1.0, None):
+        A._scale(fine, 64)
+    with pytest.raises(ValueError, match="scale must|GPU"):
+        call(scale=scale)
