@@ -376,8 +376,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<C, D, NT>::kCtasPerSm) mf_decode
                     }
                     biggest = fmaxf(biggest, __shfl_xor_sync(~0u, biggest, 1));
                     biggest = fmaxf(biggest, __shfl_xor_sync(~0u, biggest, 2));
-                    int e = (int)(__float_as_uint(biggest) >> 23) - 127;  // its exponent: scaled values lie below 2^15
-                    e = biggest == 0 || e > 127 ? 0 : e < -100 ? -100 : e;
+                    // its exponent: what is finite lies below 2^15 when scaled, also beside an infinity
+                    const int e = max(-100, min(127, (int)(__float_as_uint(biggest) >> 23) - 127));
                     const float down = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
                     up = __uint_as_float((uint32_t)(127 - 14 + e) << 23);
 #pragma unroll

@@ -37,3 +37,25 @@ def test_small_elements_beside_a_large_one(heads, dim, large, small):
     weights = 2.0 ** -11 + (2 * (dim + 2) * logit + 2 * n + 64) * u
     assert bool(((out.double() - ref).abs() <= (2.0 ** -9 * ref.abs() + weights * mass) * 1.01 + 1e-30).all())
     assert float((lse.double() - ref_lse).abs().max()) <= (2 * (dim + 2) * logit + 2 * n + 64) * u
+
+
+@pytest.mark.parametrize("cache", ["bfloat16", "float8_e4m3fn"])
+def test_an_infinite_element(cache):
+    """Every logit is infinite then: a row whose logits are all -inf has nothing to weigh, one with +inf or 0 * inf is NaN."""
+    import torch
+
+    from memfabric_hybrid_b200.ops import attention as A
+
+    data = torch.ones(4, 2, 1, 16, 64, device="cuda")
+    data[:, 0, :, :, 0] = -1
+    data[1, 0, 0, 3, 0], data[2, 0, 0, 3, 0] = 1, 0
+    data = data.to(getattr(torch, cache))
+    scales = {"k_scale": torch.ones(1, device="cuda"), "v_scale": torch.ones(1, device="cuda")} if cache == "float8_e4m3fn" else {}
+    q = torch.full((3, 2, 64), 1000.0, dtype=torch.bfloat16, device="cuda")
+    q[:, 0, 0] = float("inf")
+    q[:, 1, 0] = 1.0
+    table = torch.tensor([[0], [1], [2]], dtype=torch.int32, device="cuda")
+    lens = torch.full((3,), 16, dtype=torch.int32, device="cuda")
+    out, lse = A.decode_attention(q, data[:, 0], data[:, 1], table, lens, lse=True, **scales)
+    assert bool((out[0, 0] == 0).all()) and float(lse[0, 0]) == -float("inf")
+    assert bool(out[1:, 0].isnan().all()) and bool((out[:, 1] == 1).all())
