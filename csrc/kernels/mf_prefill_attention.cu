@@ -63,7 +63,7 @@ struct Shared {
     unsigned char kv[kStages][kTileBytes];
     uint64_t qFull, qEmpty, kvFull[kStages], kvEmpty[kStages], kvRaw[kStages], sFull[2], pFull[2], pRest[2], oFull[2], workFull[2], workEmpty[2];
     uint4 claim;  // the answer to Claim()
-    uint64_t claimed;
+    uint64_t claimed, drained;
     Work work[2], late;  // late: done clean, to get back what was taken out
     int odd[2];  // a row of the work came out infinite or NaN
     uint32_t tmem;
@@ -449,6 +449,7 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
             s.odd[i] = 0;
         }
         MbarInit(&s.claimed, 1);
+        MbarInit(&s.drained, 1);
         s.abortFlag = 0;
         MbarInitFence();
         TmaPrefetchDesc(&mapQ);
@@ -945,6 +946,15 @@ mf_prefill_attention_kernel(const __grid_constant__ CUtensorMap mapQ, const __gr
     }
     if (warp == 8) {
         TcFenceAfter();
+        if (s.abortFlag != 0) {  // products that are still under way read and write what is given back here
+            int own = 0;
+            if (ElectOne()) {
+                MmaCommit(&s.drained);
+            }
+            __syncwarp();
+            Wait(&s.drained, 0, &own);
+            TcFenceAfter();
+        }
         TmemDealloc(tmem, 512);
     }
 }
