@@ -24,7 +24,7 @@
 // A masked key counts 0 * v in a tile product, which is not 0 where v is infinite or NaN. Only the last one to three key tiles of a unit of work hold keys
 // that not all of its rows see. Where a row of such a unit comes out infinite or NaN, the unit is done once more, clean: warp 11 makes what is infinite or
 // NaN among the values of those keys 0 in shared memory before the product, and gives it back to the rows that see it behind it. What all rows see is left
-// to the product. So such a unit takes twice its time, and the others 1 to 2 % for being ready for it (cleaning all of them: 3 to 11 %).
+// to the product. So such a unit takes twice its time, and the others 1 to 2 % for being ready for it (cleaning all of them: 3 to 9 %).
 #include <cuda.h>
 
 #include <type_traits>

@@ -256,7 +256,8 @@ def prefill_attention(q, k, v, cu_q, cu_k=None, *, causal=True, scale=None, out=
 
     Returns out [tokens, heads, dim]; with lse=True (or a tensor for it) also the logarithm of the sum of exponentials, fp32
     [tokens, heads]. Rows that see no key give zeros and -inf; rows that belong to no sequence are left as they are. out must not overlap the
-    inputs. status: int32 tensor of one element, receives GEMM_PIPELINE_EXPIRED (3) if a bounded wait inside the kernel ran out."""
+    inputs. What a row may not see does not change a bit of it, NaN and infinities included. status: int32 tensor of one element, receives
+    GEMM_PIPELINE_EXPIRED (3) if a bounded wait inside the kernel ran out; rows may be unwritten then, and nothing else tells."""
     with_lse = lse is not None and lse is not False
     if lse is True or lse is False:
         lse = None
