@@ -192,3 +192,36 @@ def test_what_is_not_finite_costs_a_few_times_the_call(where):
     clean, odd = took(q, k, v), took(*bad)
     print(f"{where}: {clean * 250:.0f} us, {odd * 250:.0f} us")
     assert odd < 20 * clean, (clean, odd)
+
+
+def test_replays_and_streams_with_values_that_are_not_finite():
+    """A captured call whose values become NaN and finite again between replays, beside calls on other streams."""
+    import torch
+
+    from memfabric_hybrid_b200.ops import attention as A
+
+    cu = torch.tensor([0, 700, 701, 1900, 2000], dtype=torch.int32, device="cuda")
+    q, k, v = (_values((2100, heads, 128), torch.bfloat16, heads) for heads in (8, 2, 2))
+    odd = v.clone()
+    odd[650], odd[1300, 1, 3:40], odd[1999], odd[2000:] = float("nan"), float("inf"), float("-inf"), float("nan")
+    want = {id(x): A.prefill_attention(q, k, x, cu)[:2000].clone() for x in (v, odd)}
+    assert bool(want[id(v)].isfinite().all()) and not bool(want[id(odd)].isfinite().all())
+    taken = v.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = A.prefill_attention(q, k, taken, cu)
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    torch.cuda.synchronize()
+    for turn in range(6):
+        x = odd if turn % 2 else v
+        taken.copy_(x)
+        graph.replay()
+        for i, s in enumerate(streams):
+            y = odd if (turn + i) % 2 else v
+            got.append((A.prefill_attention(q, k, y, cu, stream=s), y))
+        torch.cuda.synchronize()
+        same = torch.equal(out[:2000].nan_to_num(5.0), want[id(x)].nan_to_num(5.0))
+        assert same
+    for z, y in got:
+        same = torch.equal(z[:2000].nan_to_num(5.0), want[id(y)].nan_to_num(5.0))
+        assert same
