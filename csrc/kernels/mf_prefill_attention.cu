@@ -315,22 +315,12 @@ struct Ranking {
     }
 };
 
+// Whether the low 16 bits are a finite T.
 template <typename T>
-struct Bits {
-    static constexpr uint32_t kExponent = Bf16<T>::value ? 0x7f80u : 0x7c00u;  // all set: infinite or NaN
-    static __device__ __forceinline__ bool Finite(uint32_t x) { return (x & kExponent) != kExponent; }
-};
-// The larger absolute values of two pairs, NaN if one is; the signs mean nothing.
-template <typename T>
-__device__ __forceinline__ uint32_t MaxAbs2(uint32_t a, uint32_t b)
+__device__ __forceinline__ bool Finite(uint32_t x)
 {
-    uint32_t r;
-    if (Bf16<T>::value) {
-        asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    } else {
-        asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    }
-    return r;
+    constexpr uint32_t kExponent = Bf16<T>::value ? 0x7f80u : 0x7c00u;
+    return (x & kExponent) != kExponent;
 }
 
 // What is infinite or NaN among the values of the keys from r0 on of a tile in shared memory becomes 0. Whole warp.
@@ -344,7 +334,7 @@ __device__ __noinline__ void Clean(unsigned char *tile, int r0)
             uint32_t *const word[4] = {&x.x, &x.y, &x.z, &x.w};
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                *word[e] &= (Bits<T>::Finite(*word[e]) ? 0xffffu : 0) | (Bits<T>::Finite(*word[e] >> 16) ? 0xffff0000u : 0);
+                *word[e] &= (Finite<T>(*word[e]) ? 0xffffu : 0) | (Finite<T>(*word[e] >> 16) ? 0xffff0000u : 0);
             }
             at[i] = x;
         }
